@@ -48,6 +48,9 @@ enum mis_dtype { MIS_F32 = 0, MIS_BF16 = 1 };
 /* region loss formed from the pooled sums: diceloss (utils/loss_fn.py:55-88) or IOULoss (:90-124) */
 enum mis_loss_kind { MIS_LOSS_DICE = 0, MIS_LOSS_IOU = 1 };
 
+/* activation of the group-norm and matrix-product entry points; MIS_ACT_GELU is the exact (error-function) form */
+enum mis_activation { MIS_ACT_NONE = 0, MIS_ACT_RELU = 1, MIS_ACT_SILU = 2, MIS_ACT_GELU = 3 };
+
 /* library / build probe */
 int         mis_version(void);              /* MAJOR*10000 + MINOR*100 + PATCH */
 const char* mis_arch(void);                 /* "gfx950" */
@@ -618,6 +621,81 @@ int mis_clip_adamw_step_dyn(const void* descs, const int* chunk_prefix, int n_te
                             int n_chunks, const void* workspace, float max_norm, double beta1, double beta2, double eps,
                             const float* step_constants, int write_clipped_grads, float* total_norm,
                             mis_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* Group norm with an activation (the reference's training default is a batch of  */
+/* 2, train.py:598-688, where batch statistics are poor; it uses nn.GroupNorm in  */
+/* model/utils/attention.py:157).  Per sample and group of C/G channels:          */
+/*   y = act((x - mean) / sqrt(var + eps) * gamma + beta)                          */
+/* x, y, dy, dx: [B][HW][C]; gamma, beta: float32 [C], NULL = 1 and 0; stats:      */
+/* float64 [B][G][2] = (mean, 1/sqrt(var+eps)), written by the forward and read    */
+/* by the backward.  dx, dgamma, dbeta may be NULL.  C % G == 0, C <= 65536,       */
+/* B and G <= 65535.  stats and workspace aligned to 16 bytes; x, y, dy, dx to     */
+/* their element (16 bytes with C a multiple of the 16-byte vector is fastest).    */
+size_t mis_group_norm_act_fwd_workspace_bytes(int dtype, int B, int64_t HW, int C, int G);
+int mis_group_norm_act_fwd(const void* x, int dtype, int B, int64_t HW, int C, int G, const float* gamma, const float* beta,
+                           double eps, int act, void* y, double* stats, void* workspace, mis_stream_t stream);
+size_t mis_group_norm_act_bwd_workspace_bytes(int dtype, int B, int64_t HW, int C, int G);
+int mis_group_norm_act_bwd(const void* x, const void* dy, int dtype, int B, int64_t HW, int C, int G, const float* gamma,
+                           const float* beta, const double* stats, int act, void* dx, float* dgamma, float* dbeta,
+                           void* workspace, mis_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* Matrix product with bias, activation and residual: y = act(x W^T + b) + r.      */
+/* x [M][K] with row stride ldx, W [N][K] dense, b float32 [N] or NULL, r [M][N]   */
+/* with row stride ldr or NULL, y [M][N] dense; strides in elements.  One element  */
+/* type for x, W, r, y; float32 accumulation.  Over the channels of a channels-last */
+/* activation (M = B*H*W) this is a 1x1 convolution (the reference's nn.Conv2d with */
+/* kernel_size=1, model/utils/modules.py:798-816).                                 */
+/* The backward forms u = x W^T + b again (only if act is not MIS_ACT_NONE):        */
+/*   dz = dy act'(u);  dx = dz W;  dw = dz^T x;  db = sum over rows of dz           */
+/* (dr is dy).  dx, dw dense in the element type, db float32; each may be NULL.     */
+/* dy has row stride ldd.  M < 2^30, N and K <= 2^20.                               */
+int mis_linear_act_fwd(const void* x, int64_t ldx, const void* w, const float* bias, const void* residual, int64_t ldr, int dtype,
+                       int64_t M, int64_t N, int64_t K, int act, void* y, mis_stream_t stream);
+size_t mis_linear_act_bwd_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K, int act);
+int mis_linear_act_bwd(const void* x, int64_t ldx, const void* w, const float* bias, const void* dy, int64_t ldd, int dtype,
+                       int64_t M, int64_t N, int64_t K, int act, void* dx, void* dw, float* db, void* workspace,
+                       mis_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* clip_grad_norm_ + AdamW.step() with both moments in 8 bits (the same update as  */
+/* mis_clip_adamw_step; the gradients are left unclipped in memory).               */
+/* descs: device array of mis_param8_desc, chunks of MIS_OPT_CHUNK elements as     */
+/* above.  The moments of all tensors live in four flat buffers: codes, one byte   */
+/* per element, and scales, one byte per 128 elements; a tensor's elements start    */
+/* at `offset`, a multiple of 128, and the codes behind its last element up to the  */
+/* next multiple of 128 are zero.  Values: exponent byte s, factor 2^(s-127);       */
+/* exp_avg code = sign, 4 exponent bits e, 3 bits f: (1 + f/8) 2^(e-15), e = 0:     */
+/* (f/8) 2^-14; exp_avg_sq = 4 bits e, 4 bits f: (1 + f/16) 2^(e-15), e = 0:        */
+/* (f/16) 2^-14.  s = 0: zeros; s = 255: not-a-number (a moment was not finite).    */
+/* Rounding to codes is stochastic: Philox4x32-10 under `seed`, counter (element    */
+/* offset / 4, step).                                                               */
+/* mis_adamw8_sqsum leaves partial sums of the gradients' squares in the workspace; */
+/* mis_adamw8_step takes them (norm_workspace) to clip to max_norm (<= 0: only the  */
+/* norm is formed) or NULL: no clipping; total_norm (may be NULL) receives the norm. */
+/* step_constants: NULL, or a device copy of what mis_adamw8_step_constants (host   */
+/* only) wrote, MIS_ADAMW8_CONSTANTS_BYTES long: lr, weight_decay and step are then  */
+/* taken from there (a launch captured once and replayed every step).               */
+/* mis_adamw8_moments writes the values of n_blocks blocks of codes.                */
+#define MIS_ADAMW8_CONSTANTS_BYTES 20
+typedef struct {
+  void* p;            /* parameter                                       */
+  const void* g;      /* gradient, same type                             */
+  int64_t offset;     /* first element in the flat moment buffers        */
+  int64_t n;          /* elements                                        */
+  int64_t dtype;      /* mis_dtype of p and g                            */
+} mis_param8_desc;
+size_t mis_adamw8_workspace_bytes(void);
+int mis_adamw8_sqsum(const void* descs, const int* chunk_prefix, int n_tensors, int n_chunks, void* workspace,
+                     mis_stream_t stream);
+int mis_adamw8_step_constants(double lr, double beta1, double beta2, double weight_decay, int64_t step, void* host_out);
+int mis_adamw8_step(const void* descs, const int* chunk_prefix, int n_tensors, int chunk_begin, int chunk_end, int n_chunks,
+                    void* exp_avg, void* exp_avg_scale, void* exp_avg_sq, void* exp_avg_sq_scale, const void* norm_workspace,
+                    double max_norm, double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step,
+                    uint64_t seed, const void* step_constants, float* total_norm, mis_stream_t stream);
+int mis_adamw8_moments(const void* exp_avg, const void* exp_avg_scale, const void* exp_avg_sq, const void* exp_avg_sq_scale,
+                       int64_t n_blocks, float* out_avg, float* out_sq, mis_stream_t stream);
 
 #ifdef __cplusplus
 }

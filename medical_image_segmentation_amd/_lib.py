@@ -106,6 +106,19 @@ PROTOTYPES = {
                                 _vp, _vp]),
     "mis_dwconv_compose_fwd": (_i, [_vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp]),
     "mis_dwconv_compose_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp]),
+    "mis_group_norm_act_fwd_workspace_bytes": (_sz, [_i, _i, _i64, _i, _i]),
+    "mis_group_norm_act_fwd": (_i, [_vp, _i, _i, _i64, _i, _i, _vp, _vp, _d, _i, _vp, _vp, _vp, _vp]),
+    "mis_group_norm_act_bwd_workspace_bytes": (_sz, [_i, _i, _i64, _i, _i]),
+    "mis_group_norm_act_bwd": (_i, [_vp, _vp, _i, _i, _i64, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp]),
+    "mis_linear_act_fwd": (_i, [_vp, _i64, _vp, _vp, _vp, _i64, _i, _i64, _i64, _i64, _i, _vp, _vp]),
+    "mis_linear_act_bwd_workspace_bytes": (_sz, [_i, _i64, _i64, _i64, _i]),
+    "mis_linear_act_bwd": (_i, [_vp, _i64, _vp, _vp, _vp, _i64, _i, _i64, _i64, _i64, _i, _vp, _vp, _vp, _vp, _vp]),
+    "mis_adamw8_workspace_bytes": (_sz, []),
+    "mis_adamw8_sqsum": (_i, [_vp, _vp, _i, _i, _vp, _vp]),
+    "mis_adamw8_step_constants": (_i, [_d, _d, _d, _d, _i64, _vp]),
+    "mis_adamw8_step": (_i, [_vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _d, _d, _d, _d, _d, _d, _i64, C.c_uint64, _vp,
+                             _vp, _vp]),
+    "mis_adamw8_moments": (_i, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp]),
     "mis_slide_gather_tiles": (_i, [_vp, _i, _i, _i, _vp, _i, _i, _i, _vp, _vp]),
     "mis_argmax_classes": (_i, [_vp, _i, _i64, _i64, _i64, _i, _i, _i, _vp, _vp]),
     "mis_slide_blend": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _i, _vp, _vp]),

@@ -1,0 +1,562 @@
+// Group norm with an activation on channels-last activations, forward and backward.
+//
+//   per sample b and group g (Cg = C/G channels, N = HW*Cg values):
+//     mean, rstd = 1/sqrt(var + eps);  xh = (x - mean) rstd;  u = xh gamma + beta;  y = act(u)
+//     du = dy act'(u);  dbeta = sum du;  dgamma = sum du xh
+//     dx = rstd (du gamma - m1 - xh m2),  m1 = sum(du gamma)/N,  m2 = sum(du gamma xh)/N
+//
+// HBM-bound: forward reads x and writes y, backward reads x and dy and writes dx.
+// A workgroup owns a range of pixels and a slab of at most 256 channel vectors that starts and ends with a group
+// (or lies inside one group, when a group is wider); a thread keeps one channel vector and walks the pixels, so a
+// wave reads contiguous memory and everything that belongs to a channel stays in registers.
+// The statistics are plain sums of x and x*x in 64 bits: on this chip a double add costs what a float add costs,
+// and 53 bits make the subtraction E[x^2] - mean^2 harmless (any spread that the input's 24 bits can hold survives).
+// Sums over pixels are combined in a fixed order: results repeat bit for bit.
+#include "act.h"
+#include "common.h"
+
+namespace {
+
+constexpr int GN_THREADS = 256;
+
+// N elements (N * sizeof(T) = 2..16 bytes, aligned to that) <-> floats
+template <typename T, int N> struct Bits;
+template <typename T> struct Bits<T, 1> { typedef T type; };
+template <> struct Bits<bf16, 2> { typedef uint32_t type; };
+template <> struct Bits<bf16, 4> { typedef uint2 type; };
+template <> struct Bits<bf16, 8> { typedef uint4 type; };
+template <> struct Bits<float, 2> { typedef uint2 type; };
+template <> struct Bits<float, 4> { typedef uint4 type; };
+
+template <typename T, int V> union Vec {
+  typename Bits<T, V>::type u;
+  T t[V];
+  __device__ Vec() {}
+};
+
+struct Shape {
+  int64_t HW;
+  int C, G, Cg;
+  int gps;          // groups per slab (1 when a group needs several slabs)
+  int parts;        // slabs per group (1 when a slab holds whole groups)
+  int slab_c;       // channels of a full slab
+  int CV, PR;       // channel vectors of a full slab, pixels side by side in a workgroup
+  int slabs, chunks;
+  int64_t ppc;      // pixels per chunk
+};
+
+struct Slab {       // of one workgroup
+  int c0, nc, g0, ng;
+};
+
+__device__ __forceinline__ Slab slab_of(const Shape& s, int i) {
+  Slab r;
+  if (s.parts == 1) {
+    r.g0 = i * s.gps;
+    r.ng = min(s.gps, s.G - r.g0);
+    r.c0 = r.g0 * s.Cg;
+    r.nc = r.ng * s.Cg;
+  } else {
+    r.g0 = i / s.parts;
+    r.ng = 1;
+    const int o = (i - r.g0 * s.parts) * s.slab_c;
+    r.c0 = r.g0 * s.Cg + o;
+    r.nc = min(s.slab_c, s.Cg - o);
+  }
+  return r;
+}
+
+// sums[b][chunk*parts + part][g] = (sum x, sum x*x) over the chunk's pixels and the slab's channels of g
+template <typename T, int V>
+__global__ __launch_bounds__(GN_THREADS) void gn_sums_kernel(const T* __restrict__ x, Shape s, double2* __restrict__ sums) {
+  extern __shared__ __attribute__((aligned(16))) char gn_lds[];
+  double2* red = (double2*)gn_lds;                       // [PR][CV*V]
+  const int b = blockIdx.z, tid = threadIdx.x;
+  const Slab sl = slab_of(s, blockIdx.y);
+  const int cv = tid % s.CV, pr = tid / s.CV;
+  const int64_t p0 = (int64_t)blockIdx.x * s.ppc, p1 = min(p0 + s.ppc, s.HW);
+  const bool on = pr < s.PR && cv * V < sl.nc;
+  double a1[V], a2[V];
+#pragma unroll
+  for (int k = 0; k < V; k++) a1[k] = a2[k] = 0.0;
+  if (on) {
+    const T* xp = x + (int64_t)b * s.HW * s.C + sl.c0 + cv * V;
+#pragma unroll 4
+    for (int64_t p = p0 + pr; p < p1; p += s.PR) {
+      Vec<T, V> v;
+      v.u = *(const typename Bits<T, V>::type*)(xp + p * s.C);
+#pragma unroll
+      for (int k = 0; k < V; k++) {
+        const double d = (double)to_f32(v.t[k]);
+        a1[k] += d;
+        a2[k] = fma(d, d, a2[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < V; k++) red[(pr * s.CV + cv) * V + k] = make_double2(a1[k], a2[k]);
+  }
+  __syncthreads();
+  const int W = s.CV * V;
+  int n = s.PR;
+  while (n > 1) {                                        // pixel rows: halves onto halves
+    const int h = (n + 1) >> 1;
+    for (int i = tid; i < (n - h) * W; i += GN_THREADS) {
+      const int r = i / W, c = i - r * W;
+      if (c < sl.nc) {
+        red[i].x += red[i + h * W].x;
+        red[i].y += red[i + h * W].y;
+      }
+    }
+    __syncthreads();
+    n = h;
+  }
+  const int part = s.parts == 1 ? 0 : blockIdx.y % s.parts;
+  double2* out = sums + ((int64_t)b * s.chunks * s.parts + (int64_t)blockIdx.x * s.parts + part) * s.G;
+  const int gc = s.parts == 1 ? s.Cg : sl.nc;
+  for (int g = tid; g < sl.ng; g += GN_THREADS) {
+    double t1 = 0.0, t2 = 0.0;
+    for (int c = 0; c < gc; c++) {
+      t1 += red[g * gc + c].x;
+      t2 += red[g * gc + c].y;
+    }
+    out[sl.g0 + g] = make_double2(t1, t2);
+  }
+}
+
+// stats[b][g] = (mean, 1/sqrt(var + eps)); one wave per (b, g)
+__global__ __launch_bounds__(64) void gn_stats_kernel(const double2* __restrict__ sums, int rows, int G, double count,
+                                                      double eps, double2* __restrict__ stats) {
+  const int g = blockIdx.x, b = blockIdx.y, lane = threadIdx.x;
+  double t1 = 0.0, t2 = 0.0;
+  for (int r = lane; r < rows; r += 64) {
+    const double2 v = sums[((int64_t)b * rows + r) * G + g];
+    t1 += v.x;
+    t2 += v.y;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    t1 += __shfl_xor(t1, o, WAVE);
+    t2 += __shfl_xor(t2, o, WAVE);
+  }
+  if (lane == 0) {
+    const double mean = t1 / count;
+    double var = t2 / count - mean * mean;
+    if (var < 0.0) var = 0.0;                            // (NaN stays NaN)
+    stats[(int64_t)b * G + g] = make_double2(mean, 1.0 / sqrt(var + eps));
+  }
+}
+
+// What a thread holds of its V channels: u = (x - mean) * a + beta, a = rstd * gamma.
+template <int V> struct Consts {
+  float mean[V], a[V], beta[V];
+};
+
+template <int V>
+__device__ __forceinline__ void load_consts(Consts<V>& k, const double2* __restrict__ stats, const float* __restrict__ gamma,
+                                            const float* __restrict__ beta, int c, int Cg) {
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    const double2 st = stats[(c + i) / Cg];
+    k.mean[i] = (float)st.x;
+    k.a[i] = (float)st.y * (gamma ? gamma[c + i] : 1.f);
+    k.beta[i] = beta ? beta[c + i] : 0.f;
+  }
+}
+
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(GN_THREADS) void gn_apply_kernel(const T* __restrict__ x, Shape s, const double2* __restrict__ stats,
+                                                              const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                              T* __restrict__ y) {
+  const int b = blockIdx.z, tid = threadIdx.x;
+  const Slab sl = slab_of(s, blockIdx.y);
+  const int cv = tid % s.CV, pr = tid / s.CV;
+  if (pr >= s.PR || cv * V >= sl.nc) return;
+  const int c = sl.c0 + cv * V;
+  Consts<V> k;
+  load_consts<V>(k, stats + (int64_t)b * s.G, gamma, beta, c, s.Cg);
+  const int64_t p0 = (int64_t)blockIdx.x * s.ppc, p1 = min(p0 + s.ppc, s.HW);
+  const int64_t base = (int64_t)b * s.HW * s.C + c;
+#pragma unroll 4
+  for (int64_t p = p0 + pr; p < p1; p += s.PR) {
+    Vec<T, V> v;
+    v.u = *(const typename Bits<T, V>::type*)(x + base + p * s.C);
+#pragma unroll
+    for (int i = 0; i < V; i++) v.t[i] = from_f32<T>(act_value<ACT>(fmaf(to_f32(v.t[i]) - k.mean[i], k.a[i], k.beta[i])));
+    *(typename Bits<T, V>::type*)(y + base + p * s.C) = v.u;
+  }
+}
+
+// du = dy act'(u).  ReLU's slope has a jump: where u is within the rounding of its float evaluation of zero (one
+// value in a million), its sign is taken from the 64-bit statistics, so that the mask is the definition's.
+template <int ACT>
+__device__ __forceinline__ float du_of(float x, float dy, float mean, float a, float beta, int c, int Cg,
+                                       const double2* __restrict__ stats, const float* __restrict__ gamma) {
+  const float u = fmaf(x - mean, a, beta);
+  if constexpr (ACT == MIS_ACT_NONE) {
+    return dy;
+  } else if constexpr (ACT == MIS_ACT_RELU) {
+    bool pos = u > 0.f;
+    if (fabsf(u) < 1e-6f * fmaf(fabsf(x) + fabsf(mean), fabsf(a), fabsf(beta))) {
+      const double2 st = stats[c / Cg];
+      pos = ((double)x - st.x) * st.y * (gamma ? (double)gamma[c] : 1.0) + (double)beta > 0.0;
+    }
+    return pos ? dy : 0.f;
+  } else {
+    return dy * act_slope<ACT>(u);
+  }
+}
+
+// rows[b][chunk][2][C] = (sum du, sum du xh) over the chunk's pixels
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(GN_THREADS) void gn_bwd_sums_kernel(const T* __restrict__ x, const T* __restrict__ dy, Shape s,
+                                                                 const double2* __restrict__ stats_all,
+                                                                 const float* __restrict__ gamma,
+                                                                 const float* __restrict__ beta, float* __restrict__ rows) {
+  extern __shared__ __attribute__((aligned(16))) char gn_lds[];
+  float2* red = (float2*)gn_lds;                         // [PR][CV*V]
+  const int b = blockIdx.z, tid = threadIdx.x;
+  const Slab sl = slab_of(s, blockIdx.y);
+  const int cv = tid % s.CV, pr = tid / s.CV;
+  const int64_t p0 = (int64_t)blockIdx.x * s.ppc, p1 = min(p0 + s.ppc, s.HW);
+  const double2* stats = stats_all + (int64_t)b * s.G;
+  if (pr < s.PR && cv * V < sl.nc) {
+    const int c = sl.c0 + cv * V;
+    Consts<V> k;
+    load_consts<V>(k, stats, gamma, beta, c, s.Cg);
+    float a1[V], a2[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) a1[i] = a2[i] = 0.f;
+    const int64_t base = (int64_t)b * s.HW * s.C + c;
+#pragma unroll 2
+    for (int64_t p = p0 + pr; p < p1; p += s.PR) {
+      Vec<T, V> vx, vd;
+      vx.u = *(const typename Bits<T, V>::type*)(x + base + p * s.C);
+      vd.u = *(const typename Bits<T, V>::type*)(dy + base + p * s.C);
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        const float xf = to_f32(vx.t[i]);
+        const float du = du_of<ACT>(xf, to_f32(vd.t[i]), k.mean[i], k.a[i], k.beta[i], c + i, s.Cg, stats, gamma);
+        a1[i] += du;
+        a2[i] = fmaf(du, xf - k.mean[i], a2[i]);         // times rstd at the end
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++)
+      red[(pr * s.CV + cv) * V + i] = make_float2(a1[i], a2[i] * (float)stats[(c + i) / s.Cg].y);
+  }
+  __syncthreads();
+  const int W = s.CV * V;
+  int n = s.PR;
+  while (n > 1) {
+    const int h = (n + 1) >> 1;
+    for (int i = tid; i < (n - h) * W; i += GN_THREADS) {
+      const int r = i / W, c = i - r * W;
+      if (c < sl.nc) {
+        red[i].x += red[i + h * W].x;
+        red[i].y += red[i + h * W].y;
+      }
+    }
+    __syncthreads();
+    n = h;
+  }
+  float* out = rows + ((int64_t)b * s.chunks + blockIdx.x) * 2 * s.C;
+  for (int c = tid; c < sl.nc; c += GN_THREADS) {
+    out[sl.c0 + c] = red[c].x;
+    out[s.C + sl.c0 + c] = red[c].y;
+  }
+}
+
+// chan[b][2][C] = sums over the chunks; dbeta, dgamma = sums over the samples.  Block (32 channels, 8 row lanes).
+__global__ __launch_bounds__(256) void gn_bwd_channels_kernel(const float* __restrict__ rows, int B, int chunks, int C,
+                                                              float* __restrict__ chan, float* __restrict__ dgamma,
+                                                              float* __restrict__ dbeta) {
+  __shared__ double2 red[8][33];
+  const int lane = threadIdx.x & 31, r = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  double s1 = 0.0, s2 = 0.0;
+  for (int b = 0; b < B; b++) {
+    double t1 = 0.0, t2 = 0.0;
+    if (c < C) {
+      const float* p = rows + (int64_t)b * chunks * 2 * C + c;
+      for (int i = r; i < chunks; i += 8) {
+        t1 += (double)p[(int64_t)i * 2 * C];
+        t2 += (double)p[(int64_t)i * 2 * C + C];
+      }
+    }
+    red[r][lane] = make_double2(t1, t2);
+    __syncthreads();
+    if (r == 0 && c < C) {
+      for (int i = 1; i < 8; i++) {
+        t1 += red[i][lane].x;
+        t2 += red[i][lane].y;
+      }
+      chan[(int64_t)b * 2 * C + c] = (float)t1;
+      chan[(int64_t)b * 2 * C + C + c] = (float)t2;
+      s1 += t1;
+      s2 += t2;
+    }
+    __syncthreads();
+  }
+  if (r == 0 && c < C) {
+    if (dbeta) dbeta[c] = (float)s1;
+    if (dgamma) dgamma[c] = (float)s2;
+  }
+}
+
+// coef[b][g] = (m1, m2): one wave per (b, g)
+__global__ __launch_bounds__(64) void gn_bwd_coef_kernel(const float* __restrict__ chan, const float* __restrict__ gamma, int C,
+                                                         int Cg, int G, double count, float2* __restrict__ coef) {
+  const int g = blockIdx.x, b = blockIdx.y;
+  const float* p = chan + (int64_t)b * 2 * C + (int64_t)g * Cg;
+  double t1 = 0.0, t2 = 0.0;
+  for (int c = threadIdx.x; c < Cg; c += 64) {
+    const double w = gamma ? (double)gamma[g * Cg + c] : 1.0;
+    t1 += w * (double)p[c];
+    t2 += w * (double)p[C + c];
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    t1 += __shfl_xor(t1, o, WAVE);
+    t2 += __shfl_xor(t2, o, WAVE);
+  }
+  if (threadIdx.x == 0) coef[(int64_t)b * G + g] = make_float2((float)(t1 / count), (float)(t2 / count));
+}
+
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(GN_THREADS) void gn_bwd_dx_kernel(const T* __restrict__ x, const T* __restrict__ dy, Shape s,
+                                                               const double2* __restrict__ stats_all,
+                                                               const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                               const float2* __restrict__ coef, T* __restrict__ dx) {
+  const int b = blockIdx.z, tid = threadIdx.x;
+  const Slab sl = slab_of(s, blockIdx.y);
+  const int cv = tid % s.CV, pr = tid / s.CV;
+  if (pr >= s.PR || cv * V >= sl.nc) return;
+  const double2* stats = stats_all + (int64_t)b * s.G;
+  const int c = sl.c0 + cv * V;
+  Consts<V> k;
+  load_consts<V>(k, stats, gamma, beta, c, s.Cg);
+  float q1[V], q2[V];                                    // dx = du a - q1 - (x - mean) q2
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    const int g = (c + i) / s.Cg;
+    const float rstd = (float)stats[g].y;
+    const float2 m = coef[(int64_t)b * s.G + g];
+    q1[i] = rstd * m.x;
+    q2[i] = rstd * rstd * m.y;
+  }
+  const int64_t p0 = (int64_t)blockIdx.x * s.ppc, p1 = min(p0 + s.ppc, s.HW);
+  const int64_t base = (int64_t)b * s.HW * s.C + c;
+#pragma unroll 2
+  for (int64_t p = p0 + pr; p < p1; p += s.PR) {
+    Vec<T, V> vx, vd;
+    vx.u = *(const typename Bits<T, V>::type*)(x + base + p * s.C);
+    vd.u = *(const typename Bits<T, V>::type*)(dy + base + p * s.C);
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      const float xf = to_f32(vx.t[i]);
+      const float du = du_of<ACT>(xf, to_f32(vd.t[i]), k.mean[i], k.a[i], k.beta[i], c + i, s.Cg, stats, gamma);
+      vd.t[i] = from_f32<T>(fmaf(du, k.a[i], -fmaf(xf - k.mean[i], q2[i], q1[i])));
+    }
+    *(typename Bits<T, V>::type*)(dx + base + p * s.C) = vd.u;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------------------
+// Slabs for vectors of V channels; false when they would not start on a vector.
+bool plan_slabs(Shape& s, int V) {
+  if (s.C % V) return false;
+  const int most = GN_THREADS * V;
+  if (s.Cg <= most) {
+    s.parts = 1;
+    s.gps = most / s.Cg;
+    if (s.gps >= s.G) {
+      s.gps = s.G;
+    } else {
+      int step = 1;                                     // groups until a slab start is a multiple of V again
+      while ((int64_t)step * s.Cg % V) step++;
+      if (s.gps < step) return false;
+      s.gps = s.gps / step * step;
+    }
+    s.slab_c = s.gps * s.Cg;
+    s.slabs = cdiv(s.G, s.gps);
+  } else {
+    if (s.Cg % V) return false;
+    s.gps = 1;
+    s.slab_c = most;
+    s.parts = cdiv(s.Cg, most);
+    s.slabs = s.G * s.parts;
+  }
+  if (s.slab_c % V) return false;
+  s.CV = s.slab_c / V;
+  s.PR = GN_THREADS / s.CV;
+  return true;
+}
+
+// The widest vector that the channel count, the slabs and the tensors' addresses allow; chunks so that the launch
+// fills the chip eight times over but a thread still walks 16 pixels.
+int plan(Shape& s, int B, int64_t HW, int C, int G, int esize, uintptr_t addr) {
+  s.HW = HW;
+  s.C = C;
+  s.G = G;
+  s.Cg = C / G;
+  int V = 16 / esize;
+  while (V > 1 && (addr % (V * esize) || !plan_slabs(s, V))) V >>= 1;
+  if (V == 1) plan_slabs(s, 1);
+  const int64_t most = (HW + (int64_t)s.PR * 16 - 1) / ((int64_t)s.PR * 16);
+  int64_t want = (2048 + (int64_t)B * s.slabs - 1) / ((int64_t)B * s.slabs);
+  if (want > most) want = most;
+  if (want < 1) want = 1;
+  s.ppc = (HW + want - 1) / want;
+  s.chunks = (int)((HW + s.ppc - 1) / s.ppc);
+  return V;
+}
+
+bool shape_ok(int dtype, int B, int64_t HW, int C, int G) {
+  return (dtype == MIS_F32 || dtype == MIS_BF16) && B >= 1 && B <= 65535 && HW >= 1 && C >= 1 && G >= 1 && C % G == 0 &&
+         C <= 65536 && G <= 65535 && HW <= ((int64_t)1 << 40);
+}
+
+template <typename T, int V>
+void launch_fwd(const T* x, const Shape& s, int B, const float* gamma, const float* beta, double eps, int act, T* y,
+                double2* stats, double2* sums, hipStream_t st) {
+  const dim3 grid(s.chunks, s.slabs, B);
+  const size_t lds = (size_t)s.PR * s.CV * V * sizeof(double2);
+  gn_sums_kernel<T, V><<<grid, GN_THREADS, lds, st>>>(x, s, sums);
+  gn_stats_kernel<<<dim3(s.G, B), 64, 0, st>>>(sums, s.chunks * s.parts, s.G, (double)s.HW * s.Cg, eps, stats);
+  switch (act) {
+    case MIS_ACT_RELU: gn_apply_kernel<T, V, MIS_ACT_RELU><<<grid, GN_THREADS, 0, st>>>(x, s, stats, gamma, beta, y); break;
+    case MIS_ACT_SILU: gn_apply_kernel<T, V, MIS_ACT_SILU><<<grid, GN_THREADS, 0, st>>>(x, s, stats, gamma, beta, y); break;
+    case MIS_ACT_GELU: gn_apply_kernel<T, V, MIS_ACT_GELU><<<grid, GN_THREADS, 0, st>>>(x, s, stats, gamma, beta, y); break;
+    default: gn_apply_kernel<T, V, MIS_ACT_NONE><<<grid, GN_THREADS, 0, st>>>(x, s, stats, gamma, beta, y);
+  }
+}
+
+struct BwdBuffers {
+  float *rows, *chan;
+  float2* coef;
+};
+
+template <typename T, int V, int ACT>
+void launch_bwd_act(const T* x, const T* dy, const Shape& s, int B, const float* gamma, const float* beta,
+                    const double2* stats, T* dx, float* dgamma, float* dbeta, const BwdBuffers& w, hipStream_t st) {
+  const dim3 grid(s.chunks, s.slabs, B);
+  const size_t lds = (size_t)s.PR * s.CV * V * sizeof(float2);
+  gn_bwd_sums_kernel<T, V, ACT><<<grid, GN_THREADS, lds, st>>>(x, dy, s, stats, gamma, beta, w.rows);
+  gn_bwd_channels_kernel<<<cdiv(s.C, 32), 256, 0, st>>>(w.rows, B, s.chunks, s.C, w.chan, dgamma, dbeta);
+  if (!dx) return;
+  gn_bwd_coef_kernel<<<dim3(s.G, B), 64, 0, st>>>(w.chan, gamma, s.C, s.Cg, s.G, (double)s.HW * s.Cg, w.coef);
+  gn_bwd_dx_kernel<T, V, ACT><<<grid, GN_THREADS, 0, st>>>(x, dy, s, stats, gamma, beta, w.coef, dx);
+}
+
+template <typename T, int V>
+void launch_bwd(const T* x, const T* dy, const Shape& s, int B, const float* gamma, const float* beta, int act,
+                const double2* stats, T* dx, float* dgamma, float* dbeta, const BwdBuffers& w, hipStream_t st) {
+  switch (act) {
+    case MIS_ACT_RELU: launch_bwd_act<T, V, MIS_ACT_RELU>(x, dy, s, B, gamma, beta, stats, dx, dgamma, dbeta, w, st); break;
+    case MIS_ACT_SILU: launch_bwd_act<T, V, MIS_ACT_SILU>(x, dy, s, B, gamma, beta, stats, dx, dgamma, dbeta, w, st); break;
+    case MIS_ACT_GELU: launch_bwd_act<T, V, MIS_ACT_GELU>(x, dy, s, B, gamma, beta, stats, dx, dgamma, dbeta, w, st); break;
+    default: launch_bwd_act<T, V, MIS_ACT_NONE>(x, dy, s, B, gamma, beta, stats, dx, dgamma, dbeta, w, st);
+  }
+}
+
+// Calls f(pointer type tag, vector width) for the planned width.
+template <typename F>
+void with_vector(int dtype, int V, F&& f) {
+  if (dtype == MIS_BF16) {
+    if (V == 8) f((bf16*)nullptr, std::integral_constant<int, 8>());
+    else if (V == 4) f((bf16*)nullptr, std::integral_constant<int, 4>());
+    else if (V == 2) f((bf16*)nullptr, std::integral_constant<int, 2>());
+    else f((bf16*)nullptr, std::integral_constant<int, 1>());
+  } else {
+    if (V == 4) f((float*)nullptr, std::integral_constant<int, 4>());
+    else if (V == 2) f((float*)nullptr, std::integral_constant<int, 2>());
+    else f((float*)nullptr, std::integral_constant<int, 1>());
+  }
+}
+
+// Workspace sizes hold for every vector width (a tensor's address may rule the widest out).
+size_t fwd_bytes(int dtype, int B, int64_t HW, int C, int G) {
+  size_t most = 0;
+  for (uintptr_t addr = 2; addr <= 16; addr *= 2) {
+    Shape s;
+    plan(s, B, HW, C, G, dtype == MIS_BF16 ? 2 : 4, addr);
+    const size_t n = (size_t)B * s.chunks * s.parts * s.G * sizeof(double2);
+    if (n > most) most = n;
+  }
+  return align256(most);
+}
+
+size_t bwd_rows_bytes(int dtype, int B, int64_t HW, int C, int G) {
+  size_t most = 0;
+  for (uintptr_t addr = 2; addr <= 16; addr *= 2) {
+    Shape s;
+    plan(s, B, HW, C, G, dtype == MIS_BF16 ? 2 : 4, addr);
+    const size_t n = (size_t)B * s.chunks * 2 * C * sizeof(float);
+    if (n > most) most = n;
+  }
+  return align256(most);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t mis_group_norm_act_fwd_workspace_bytes(int dtype, int B, int64_t HW, int C, int G) {
+  return shape_ok(dtype, B, HW, C, G) ? fwd_bytes(dtype, B, HW, C, G) : 0;
+}
+
+int mis_group_norm_act_fwd(const void* x, int dtype, int B, int64_t HW, int C, int G, const float* gamma, const float* beta,
+                           double eps, int act, void* y, double* stats, void* workspace, mis_stream_t stream) {
+  MIS_REQUIRE(x && y && stats && workspace, "group_norm_act_fwd: null pointer");
+  MIS_REQUIRE(shape_ok(dtype, B, HW, C, G), "group_norm_act_fwd: bad dtype or shape (B=%d HW=%lld C=%d groups=%d)", B,
+              (long long)HW, C, G);
+  MIS_REQUIRE(act >= MIS_ACT_NONE && act <= MIS_ACT_GELU, "group_norm_act_fwd: unknown activation %d", act);
+  MIS_REQUIRE(eps >= 0.0, "group_norm_act_fwd: eps must not be negative");
+  MIS_REQUIRE((((uintptr_t)x | (uintptr_t)y) & (dtype == MIS_BF16 ? 1 : 3)) == 0 &&
+              (((uintptr_t)stats | (uintptr_t)workspace) & 15) == 0, "group_norm_act_fwd: misaligned pointer");
+  Shape s;
+  const int V = plan(s, B, HW, C, G, dtype == MIS_BF16 ? 2 : 4, (uintptr_t)x | (uintptr_t)y | 16);
+  with_vector(dtype, V, [&](auto* t, auto v) {
+    typedef std::remove_pointer_t<decltype(t)> T;
+    launch_fwd<T, decltype(v)::value>((const T*)x, s, B, gamma, beta, eps, act, (T*)y, (double2*)stats, (double2*)workspace,
+                                      (hipStream_t)stream);
+  });
+  MIS_CHECK_LAUNCH("group_norm_act_fwd");
+  return MIS_OK;
+}
+
+size_t mis_group_norm_act_bwd_workspace_bytes(int dtype, int B, int64_t HW, int C, int G) {
+  if (!shape_ok(dtype, B, HW, C, G)) return 0;
+  return bwd_rows_bytes(dtype, B, HW, C, G) + align256((size_t)B * 2 * C * sizeof(float)) +
+         align256((size_t)B * G * sizeof(float2));
+}
+
+int mis_group_norm_act_bwd(const void* x, const void* dy, int dtype, int B, int64_t HW, int C, int G, const float* gamma,
+                           const float* beta, const double* stats, int act, void* dx, float* dgamma, float* dbeta,
+                           void* workspace, mis_stream_t stream) {
+  MIS_REQUIRE(x && dy && stats && workspace, "group_norm_act_bwd: null pointer");
+  MIS_REQUIRE(shape_ok(dtype, B, HW, C, G), "group_norm_act_bwd: bad dtype or shape (B=%d HW=%lld C=%d groups=%d)", B,
+              (long long)HW, C, G);
+  MIS_REQUIRE(act >= MIS_ACT_NONE && act <= MIS_ACT_GELU, "group_norm_act_bwd: unknown activation %d", act);
+  MIS_REQUIRE((((uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx) & (dtype == MIS_BF16 ? 1 : 3)) == 0 &&
+              (((uintptr_t)stats | (uintptr_t)workspace) & 15) == 0, "group_norm_act_bwd: misaligned pointer");
+  Shape s;
+  const int V = plan(s, B, HW, C, G, dtype == MIS_BF16 ? 2 : 4, (uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx | 16);
+  BwdBuffers w;
+  char* ws = (char*)workspace;
+  w.rows = (float*)ws;
+  ws += bwd_rows_bytes(dtype, B, HW, C, G);
+  w.chan = (float*)ws;
+  ws += align256((size_t)B * 2 * C * sizeof(float));
+  w.coef = (float2*)ws;
+  with_vector(dtype, V, [&](auto* t, auto v) {
+    typedef std::remove_pointer_t<decltype(t)> T;
+    launch_bwd<T, decltype(v)::value>((const T*)x, (const T*)dy, s, B, gamma, beta, act, (const double2*)stats, (T*)dx,
+                                      dgamma, dbeta, w, (hipStream_t)stream);
+  });
+  MIS_CHECK_LAUNCH("group_norm_act_bwd");
+  return MIS_OK;
+}
+
+}  // extern "C"

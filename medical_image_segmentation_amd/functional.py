@@ -1834,3 +1834,186 @@ class ChannelScaleFn(torch.autograd.Function):
                 call("mis_channel_dot", x.data_ptr(), dout.data_ptr(), _dt(x), B, H * W, Cc, ds.data_ptr(),
                      ws.data_ptr(), _stream())
         return dx, ds
+
+
+# ---------------------------------------------------------------------------
+# group norm with an activation; matrix product with bias, activation and residual
+# ---------------------------------------------------------------------------
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}          # mis_activation; gelu is the error-function form
+
+
+def _act_id(name):
+    try:
+        return ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"unknown activation {name!r}: one of {', '.join(ACTIVATIONS)}") from None
+
+
+class _on_device_of:
+    """The launches below go to the current stream of the tensor's own device, whichever device is current."""
+
+    def __init__(self, t):
+        self.guard = torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+def _scratch(nbytes, device):
+    """`workspace`, except while a HIP graph is being captured: scratch then comes from that graph's own pool, so that
+    two captured graphs never share a buffer."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+    return workspace(nbytes, device)
+
+
+def _check_param(t, n, name, like):
+    if t is None:
+        return
+    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{name}: expected float32 [{n}], got {t.dtype} {tuple(t.shape)}")
+    if t.device != like.device:
+        raise RuntimeError(f"{name} is on {t.device}, the input on {like.device}")
+
+
+class GroupNormActFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act):
+        B, Cc, H, W = x.shape
+        weight = weight.contiguous() if weight is not None else None
+        bias = bias.contiguous() if bias is not None else None
+        y = torch.empty_like(x, memory_format=torch.channels_last)
+        stats = torch.empty((B, groups, 2), dtype=torch.float64, device=x.device)
+        if x.numel():
+            with _on_device_of(x), _prof("group_norm_act_fwd", 8 * x.numel(), 2 * x.numel() * x.element_size()):
+                ws = _scratch(query("mis_group_norm_act_fwd_workspace_bytes", _dt(x), B, H * W, Cc, groups), x.device)
+                call("mis_group_norm_act_fwd", x.data_ptr(), _dt(x), B, H * W, Cc, groups, _p(weight), _p(bias), eps, act,
+                     y.data_ptr(), stats.data_ptr(), ws.data_ptr(), _stream())
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.groups, ctx.act = groups, act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, stats = ctx.saved_tensors
+        B, Cc, H, W = x.shape
+        dy = to_act(dy, x.dtype) if x.numel() else dy
+        dx = torch.empty_like(x, memory_format=torch.channels_last) if ctx.needs_input_grad[0] else None
+        grad = torch.empty if x.numel() else torch.zeros
+        dw = grad(Cc, dtype=torch.float32, device=x.device) if ctx.needs_input_grad[1] else None
+        db = grad(Cc, dtype=torch.float32, device=x.device) if ctx.needs_input_grad[2] else None
+        if x.numel():
+            with _on_device_of(x), _prof("group_norm_act_bwd", 22 * x.numel(), 3 * x.numel() * x.element_size()):
+                ws = _scratch(query("mis_group_norm_act_bwd_workspace_bytes", _dt(x), B, H * W, Cc, ctx.groups), x.device)
+                call("mis_group_norm_act_bwd", x.data_ptr(), dy.data_ptr(), _dt(x), B, H * W, Cc, ctx.groups, _p(weight),
+                     _p(bias), stats.data_ptr(), ctx.act, _p(dx), _p(dw), _p(db), ws.data_ptr(), _stream())
+        return dx, dw, db, None, None, None
+
+
+def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="none"):
+    """act(group_norm(x) * weight + bias) for a channels-last activation [B, C, H, W] (float32 or bfloat16), over
+    `num_groups` groups of C / num_groups channels per sample; weight and bias float32 [C] or None.  activation: "none",
+    "relu", "silu" or "gelu".  Differentiable (once) in x, weight and bias.  The statistics are kept in 64 bits."""
+    act = _act_id(activation)
+    _dt(_check_act(x))
+    if not isinstance(num_groups, int) or num_groups < 1 or x.shape[1] < 1 or x.shape[1] % num_groups:
+        raise ValueError(f"{x.shape[1]} channels cannot be split into {num_groups} groups")
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    _check_param(weight, x.shape[1], "weight", x)
+    _check_param(bias, x.shape[1], "bias", x)
+    return GroupNormActFn.apply(x, weight, bias, num_groups, float(eps), act)
+
+
+def _as_rows(t, n):
+    """[..., n] -> ([rows, n] with contiguous rows, row stride); a copy only where the strides need one."""
+    t = t.reshape(-1, n)
+    if t.stride(1) != 1 and n > 1 or t.shape[0] > 1 and t.stride(0) < n:
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else n)
+
+
+class LinearActFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        N, K = weight.shape
+        w = weight.contiguous()
+        bias = bias.contiguous() if bias is not None else None
+        x2, ldx = _as_rows(x, K)
+        r2, ldr = _as_rows(residual, N) if residual is not None else (None, 0)
+        M = x2.shape[0]
+        y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
+        if M:
+            nbytes = (M * K + N * K + M * N * (1 if r2 is None else 2)) * x.element_size()
+            with _on_device_of(x), _prof("linear_act_fwd", 2 * M * N * K, nbytes):
+                call("mis_linear_act_fwd", x2.data_ptr(), ldx, w.data_ptr(), _p(bias), _p(r2), ldr, _dt(x), M, N, K, act,
+                     y.data_ptr(), _stream())
+        ctx.save_for_backward(x, w, bias)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, bias = ctx.saved_tensors
+        N, K = w.shape
+        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+        dr = dy if need_r else None
+        if not (need_x or need_w or need_b):
+            return None, None, None, dr, None
+        x2, ldx = _as_rows(x, K)
+        d2, ldd = _as_rows(dy.to(x.dtype), N)
+        M = x2.shape[0]
+        grad = torch.empty if M else torch.zeros
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+        dw = grad((N, K), dtype=x.dtype, device=x.device) if need_w else None
+        db = grad(N, dtype=torch.float32, device=x.device) if need_b else None
+        if M:
+            nbytes = (2 * M * K + 2 * N * K + M * N) * x.element_size()
+            with _on_device_of(x), _prof("linear_act_bwd", 4 * M * N * K, nbytes):
+                ws = _scratch(query("mis_linear_act_bwd_workspace_bytes", _dt(x), M, N, K, ctx.act), x.device)
+                call("mis_linear_act_bwd", x2.data_ptr(), ldx, w.data_ptr(), _p(bias), d2.data_ptr(), ldd, _dt(x), M, N, K,
+                     ctx.act, _p(dx), _p(dw), _p(db), ws.data_ptr(), _stream())
+        return dx, dw, db, dr, None
+
+
+def linear_act(x, weight, bias=None, activation="none", residual=None):
+    """act(x @ weight.T + bias) + residual.  x [..., K], weight [N, K] and residual [..., N] in one type (float32 or
+    bfloat16), bias float32 [N]; activation "none", "relu", "silu" or "gelu".  Accumulation is float32, one rounding at
+    the end.  Differentiable (once) in all four; the backward forms the pre-activation again instead of keeping it, and
+    rounds the gradient before the activation to the tensors' type."""
+    act = _act_id(activation)
+    if not x.is_cuda:
+        raise RuntimeError(f"x: the MI355X kernels need a CUDA/HIP tensor, got {x.device} (there is no CPU fallback)")
+    _dt(x)
+    if weight.dim() != 2 or x.dim() < 1 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
+        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)}: expected [..., K] and [N, K]")
+    for t, name in ((weight, "weight"), (residual, "residual")):
+        if t is None:
+            continue
+        if t.dtype != x.dtype:
+            raise TypeError(f"{name} is {t.dtype}, x is {x.dtype}: one type for both")
+        if t.device != x.device:
+            raise RuntimeError(f"{name} is on {t.device}, x on {x.device}")
+    if residual is not None and residual.shape != x.shape[:-1] + (weight.shape[0],):
+        raise ValueError(f"residual {tuple(residual.shape)}: expected {tuple(x.shape[:-1]) + (weight.shape[0],)}")
+    _check_param(bias, weight.shape[0], "bias", x)
+    return LinearActFn.apply(x, weight, bias, residual, act)
+
+
+def pointwise_conv_act(x, weight, bias=None, activation="none", residual=None):
+    """linear_act over the channels of channels-last activations: act(conv1x1(x) + bias) + residual.  x [B, Cin, H, W],
+    residual [B, Cout, H, W], weight [Cout, Cin] or nn.Conv2d's [Cout, Cin, 1, 1]."""
+    _check_act(x)
+    if weight.dim() == 4 and tuple(weight.shape[2:]) == (1, 1):
+        weight = weight.reshape(weight.shape[:2])
+    if residual is not None:
+        residual = _check_act(residual, "residual").permute(0, 2, 3, 1)
+    return linear_act(x.permute(0, 2, 3, 1), weight, bias, activation, residual).permute(0, 3, 1, 2)

@@ -199,3 +199,55 @@ class ResDConv(nn.Module):
 
     def _initialize_weights(self, init_gain=0.02):
         _init_like_reference(self)
+
+
+class GroupNormAct(nn.GroupNorm):
+    """nn.GroupNorm followed by an activation ("none", "relu", "silu", "gelu") in the same kernels; nn.GroupNorm's
+    parameters and state_dict keys."""
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, activation="relu"):
+        super().__init__(num_groups, num_channels, eps=eps, affine=affine)
+        F_._act_id(activation)
+        self.activation = activation
+
+    def forward(self, x):
+        """x: [B, C, H, W] tensor on the GPU (float32 or bfloat16) -> a channels-last activation."""
+        return F_.group_norm_act(F_.to_act(x), self.num_groups, self.weight, self.bias, self.eps, self.activation)
+
+    def extra_repr(self):
+        return super().extra_repr() + f", activation={self.activation}"
+
+
+class PointwiseConvAct(nn.Conv2d):
+    """A 1x1 nn.Conv2d (its parameters and state_dict keys, float32) with an activation and an optional residual added
+    to the result, as one matrix product over the pixels in the type of its input."""
+
+    def __init__(self, in_channels, out_channels, bias=True, activation="none"):
+        super().__init__(in_channels, out_channels, kernel_size=1, bias=bias)
+        F_._act_id(activation)
+        self.activation = activation
+
+    def forward(self, x, residual=None):
+        x = F_.to_act(x)
+        if residual is not None:
+            residual = F_.to_act(residual, x.dtype)
+        return F_.pointwise_conv_act(x, self.weight.to(x.dtype), self.bias, self.activation, residual)
+
+    def extra_repr(self):
+        return super().extra_repr() + f", activation={self.activation}"
+
+
+class ChannelMLP(nn.Module):
+    """Residual channel mixing for small batches: x + narrow(act(widen(norm(x)))), with a group norm (statistics per
+    sample) and two 1x1 convs over `expansion` times the channels."""
+
+    def __init__(self, channels, expansion=4, num_groups=32, activation="gelu"):
+        super().__init__()
+        self.norm = GroupNormAct(num_groups, channels, activation="none")
+        self.widen = PointwiseConvAct(channels, channels * expansion, activation=activation)
+        self.narrow = PointwiseConvAct(channels * expansion, channels)
+        _init_like_reference(self)
+
+    def forward(self, x):
+        x = F_.to_act(x)
+        return self.narrow(self.widen(self.norm(x)), residual=x)

@@ -20,7 +20,7 @@ Single-process only: a gradient exchange inside the captured region is not suppo
 import torch
 
 from .. import functional as F_
-from .optim import CapturedStep, clip_and_step
+from .optim import captured_step, clip_and_step
 
 
 class GraphedTrainStep:
@@ -54,7 +54,7 @@ class GraphedTrainStep:
                 clip_and_step(optimizer, self.params, max_norm)
         torch.cuda.current_stream(images.device).wait_stream(side)
         self.steps_taken = warmup
-        self.captured = CapturedStep(optimizer, self.params, max_norm)
+        self.captured = captured_step(optimizer, self.params, max_norm)
         optimizer.zero_grad(set_to_none=True)
         torch._C._increment_version(self.params)     # the capture must contain the weight re-packing
         torch.cuda.synchronize(images.device)

@@ -7,6 +7,9 @@ The reference's step is `torch.nn.utils.clip_grad_norm_(model.parameters(), 1.0)
 interchangeable with torch's.  Anything it does not recognise — another optimizer class,
 amsgrad/maximize/capturable, sparse or non-float32 tensors, an enabled GradScaler — runs
 torch's own `clip_grad_norm_` + `optimizer.step()` unchanged.
+
+`AdamW8` is the same update with both moments in 8 bits (2.02 bytes of state per parameter instead of 8);
+`clip_and_step` and `CapturedStep` take it as they take torch's AdamW.
 """
 import torch
 
@@ -123,6 +126,12 @@ def clip_and_step(optimizer, params, max_norm=1.0):
     0-dim tensor), like clip_grad_norm_."""
     params = [p for p in params]
     F_.flush_wgrad_reduces()       # (a no-op after a finished backward pass)
+    if isinstance(optimizer, AdamW8):
+        if {id(p) for p in params if p.grad is not None} != {id(p) for p in optimizer._stepped()}:
+            norm = torch.nn.utils.clip_grad_norm_(params, max_norm=max_norm)   # a norm over other tensors than are stepped
+            optimizer.step()
+            return norm
+        return optimizer._launch(float(max_norm))
     fast = _fast_path(optimizer, params)
     if fast is not None:
         return _launch(optimizer, fast, max_norm)
@@ -224,6 +233,312 @@ def _clip_and_step_checked(optimizer, params, max_norm):
     f.step = float(steps[0] - 1)
     _FAST[id(optimizer)] = f
     return _launch(optimizer, f, max_norm)
+
+
+BLOCK8 = 128          # elements that share a scale in AdamW8's moments
+
+
+def _blocks(n):
+    return (n + BLOCK8 - 1) // BLOCK8
+
+
+def _dense(t):
+    """Whether the elements fill their memory without gaps, in whatever order."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if st != want:
+            return False
+        want *= n
+    return True
+
+
+class AdamW8(torch.optim.Optimizer):
+    """AdamW with both moments in 8 bits, one launch for all tensors (two when the gradient norm is clipped).
+
+    The update is torch.optim.AdamW's; what is kept between steps is rounded to codes of one byte with an exponent byte
+    per 128 elements (mis_adamw8_step in include/misamd.h gives the formats), stochastically: `seed` and the step number
+    decide every rounding, so runs repeat bit for bit.  Parameters float32 or bfloat16 with gradients of the same type, on
+    one GPU.  Gradients are read, not changed, when clipping (torch's clip_grad_norm_ scales them in place).  A moment
+    that is not finite makes its block of 128 read back as NaN.
+
+    state[p] = {"step": int, "exp_avg", "exp_avg_sq": uint8 codes, padded to a multiple of 128,
+                "exp_avg_scale", "exp_avg_sq_scale": uint8, one per 128}; `moments(p)` gives their float32 values.
+    The codes follow the elements' order in memory.  A parameter without a gradient is left alone, as in torch.
+    """
+    _STATE = ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale")
+    _plan = None
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, seed=0):
+        if not 0.0 <= lr:
+            raise ValueError(f"Invalid learning rate: {lr}")
+        if not 0.0 <= eps:
+            raise ValueError(f"Invalid epsilon value: {eps}")
+        if not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"Invalid betas: {betas}")
+        if not 0.0 <= weight_decay:
+            raise ValueError(f"Invalid weight_decay value: {weight_decay}")
+        if not 0 <= int(seed) < 1 << 64:
+            raise ValueError(f"Invalid seed: {seed}")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, seed=int(seed)))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dtype not in F_._DT:
+                self.param_groups.pop()
+                raise TypeError(f"AdamW8 takes float32 and bfloat16 parameters, got {p.dtype}")
+        self._plan = None
+
+    def load_state_dict(self, state_dict):
+        n = {i: p.numel() for i, p in enumerate(q for g in self.param_groups for q in g["params"])}
+        for i, s in state_dict["state"].items():
+            for k in self._STATE:
+                if k not in s:
+                    raise ValueError(f"not an AdamW8 state: parameter {i} has no {k}")
+                want = _blocks(n[i]) * (1 if k.endswith("_scale") else BLOCK8) if i in n else None
+                if want is not None and (s[k].dtype != torch.uint8 or s[k].numel() != want):
+                    raise ValueError(f"parameter {i}: {k} should be {want} bytes, got {s[k].numel()} of {s[k].dtype}")
+        super().load_state_dict(state_dict)        # (casts to the parameter's type, which holds 0..255 exactly)
+        for s in self.state.values():
+            for k in self._STATE:
+                s[k] = s[k].to(torch.uint8).reshape(-1)
+            s["step"] = int(s["step"])
+        self._plan = None
+
+    def _stepped(self):
+        return [p for g in self.param_groups for p in g["params"] if p.grad is not None]
+
+    def _flat(self):
+        """The flat moment buffers, laid out over all parameters; state[p] holds views of them."""
+        params = [p for g in self.param_groups for p in g["params"]]
+        plan = self._plan
+        if plan is not None and plan.matches(params, self.state):
+            return plan
+        devs = {p.device for p in params}
+        if len(devs) != 1 or next(iter(devs)).type != "cuda":
+            raise RuntimeError(f"AdamW8 needs all parameters on one GPU, got {sorted(map(str, devs))}")
+        plan = self._plan = _Plan8(params, next(iter(devs)))
+        for p, (b0, b1) in zip(params, plan.spans):
+            s, old = self.state[p], dict(self.state[p])
+            for k, buf in zip(self._STATE, plan.buffers):
+                w = 1 if k.endswith("_scale") else BLOCK8
+                s[k] = buf[b0 * w:b1 * w]
+                if k in old:
+                    s[k].copy_(old[k])
+            s["step"] = int(old.get("step", 0))
+        return plan
+
+    def moments(self, p=None):
+        """(exp_avg, exp_avg_sq) of parameter `p` as float32 tensors of its shape; without `p` the flat buffers of all
+        parameters in their order, each parameter starting at a multiple of 128 (zeros behind its last element)."""
+        plan = self._flat()
+        dev = plan.device
+        b0, b1 = (0, plan.blocks) if p is None else plan.spans[[id(q) for q in plan.params].index(id(p))]
+        out = [torch.empty((b1 - b0) * BLOCK8, dtype=torch.float32, device=dev) for _ in range(2)]
+        if b1 > b0:
+            m, ms, v, vs = plan.buffers
+            with F_._on_device_of(out[0]):
+                call("mis_adamw8_moments", m[b0 * BLOCK8:].data_ptr(), ms[b0:].data_ptr(), v[b0 * BLOCK8:].data_ptr(),
+                     vs[b0:].data_ptr(), b1 - b0, out[0].data_ptr(), out[1].data_ptr(), F_._stream())
+        if p is None:
+            return out[0], out[1]
+        return tuple(torch.as_strided(t, p.shape, p.stride()).clone(memory_format=torch.preserve_format) for t in out)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        self._launch(None)
+        return loss
+
+    @torch.no_grad()
+    def _launch(self, max_norm):
+        """One step; max_norm None: no norm is formed.  Returns the total gradient norm otherwise."""
+        params = self._stepped()
+        if not params:
+            return torch.zeros(()) if max_norm is not None else None
+        if params[0].is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("an AdamW8 step cannot be captured as it is (its step number would be frozen): use "
+                               "CapturedStep or GraphedTrainStep")
+        plan = self._flat()
+        table = plan.table(self.param_groups, self.state)
+        with F_._on_device_of(plan.buffers[0]):
+            st = F_._stream()
+            norm = plan.sqsum(table, st) if max_norm is not None else None
+            for k, (g, ps, c0, c1) in enumerate(table.runs):
+                b1, b2 = g["betas"]
+                plan.step(table, g, c0, c1, max_norm, float(g["lr"]), b1, b2, float(g["weight_decay"]),
+                          self.state[ps[0]]["step"] + 1, None, norm if k == 0 else None, st)
+        for p in params:
+            self.state[p]["step"] += 1
+        torch._C._increment_version(params)
+        return norm
+
+
+class _Plan8:
+    """The flat moment buffers of one AdamW8 and the device tables of its launches."""
+
+    def __init__(self, params, device):
+        self.params, self.device = params, device
+        self.spans, at = [], 0
+        for p in params:
+            if not _dense(p):
+                raise RuntimeError(f"AdamW8 needs dense parameters, got strides {p.stride()} for {tuple(p.shape)}")
+            self.spans.append((at, at + _blocks(p.numel())))
+            at = self.spans[-1][1]
+        self.blocks = at
+        self.buffers = [torch.zeros(max(at, 1) * w, dtype=torch.uint8, device=device) for w in (BLOCK8, 1, BLOCK8, 1)]
+        self.norm_ws = torch.empty(query("mis_adamw8_workspace_bytes"), dtype=torch.uint8, device=device)
+        self.tables = {}
+
+    def matches(self, params, state):
+        if len(params) != len(self.params) or any(a is not b for a, b in zip(params, self.params)):
+            return False
+        base = self.buffers[0].data_ptr()
+        return all("exp_avg" in state[p] and state[p]["exp_avg"].data_ptr() == base + b0 * BLOCK8 and p.device == self.device
+                   for p, (b0, b1) in zip(params, self.spans) if b1 > b0)
+
+    def rows(self, params):
+        """Pointer rows; a gradient in another memory order than its parameter is copied into the parameter's."""
+        span = {id(p): s for p, s in zip(self.params, self.spans)}
+        rows, keep = [], []
+        for p in params:
+            g = p.grad
+            if g.is_sparse or g.dtype != p.dtype or g.device != p.device:
+                raise RuntimeError(f"AdamW8 needs dense gradients of the parameter's type and device, got {g.dtype} "
+                                   f"{g.layout} on {g.device}")
+            if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
+                g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
+                keep.append(g)
+            rows.append((p.data_ptr(), g.data_ptr(), span[id(p)][0] * BLOCK8, p.numel(), F_._DT[p.dtype]))
+        return rows, keep
+
+    def table(self, groups, state):
+        """The launch tables for the parameters that have a gradient now: pointer rows, and runs (group, parameters,
+        first chunk, end chunk) of one group and one step number, each of them a launch."""
+        runs, order = [], []
+        for g in groups:
+            by_step = {}
+            for p in g["params"]:
+                if p.grad is not None and p.numel():
+                    by_step.setdefault(state[p]["step"], []).append(p)
+            for ps in by_step.values():
+                runs.append((g, ps))
+                order += ps
+        rows, keep = self.rows(order)
+        sizes = tuple(r[3] for r in rows)
+        t = self.tables.get(sizes)
+        if t is None:
+            if len(self.tables) >= 8:             # (a few patterns of missing gradients at most; not a growing cache)
+                self.tables.clear()
+            prefix = [0]
+            for n in sizes:
+                prefix.append(prefix[-1] + (n + CHUNK - 1) // CHUNK)
+            t = self.tables[sizes] = _Plan(sizes, None, prefix, self.device)
+        if order and t.rows != rows:
+            t.upload(rows)
+        t.keep = keep                              # (alive until the next step's table replaces them)
+        t.runs, c = [], 0
+        for g, ps in runs:
+            c0 = c
+            for p in ps:
+                c += (p.numel() + CHUNK - 1) // CHUNK
+            t.runs.append((g, ps, c0, c))
+        return t
+
+    def sqsum(self, table, st, descs=None, ws=None):
+        ws = self.norm_ws if ws is None else ws
+        if not table.n_chunks:
+            return torch.zeros((), dtype=torch.float32, device=self.device)
+        call("mis_adamw8_sqsum", (table.descs if descs is None else descs).data_ptr(), table.prefix.data_ptr(),
+             len(table.sizes), table.n_chunks, ws.data_ptr(), st)
+        return torch.empty((), dtype=torch.float32, device=self.device)
+
+    def step(self, table, g, c0, c1, max_norm, lr, b1, b2, wd, step, dyn, norm, st, descs=None, ws=None):
+        ws = self.norm_ws if ws is None else ws
+        m, ms, v, vs = self.buffers
+        call("mis_adamw8_step", (table.descs if descs is None else descs).data_ptr(), table.prefix.data_ptr(),
+             len(table.sizes), c0, c1, table.n_chunks, m.data_ptr(), ms.data_ptr(), v.data_ptr(), vs.data_ptr(),
+             ws.data_ptr() if max_norm is not None else None, 0.0 if max_norm is None else max_norm, lr, float(b1), float(b2),
+             float(g["eps"]), wd, step, g["seed"], F_._p(dyn), F_._p(norm), st)
+
+
+class _CapturedStep8:
+    """CapturedStep for an AdamW8: learning rate, weight decay and step number come from a device buffer; the norm's
+    partial sums, the pointer table and the constants belong to this object alone."""
+    RING, WIDTH = 8, 32           # bytes per run's constants (20 used)
+
+    def __init__(self, optimizer, params, max_norm):
+        params = list(params)
+        if {id(p) for p in params if p.grad is not None} != {id(p) for p in optimizer._stepped()} or not params:
+            raise RuntimeError("CapturedStep needs the gradients of exactly the tensors that the optimizer steps")
+        if any(optimizer.state[p].get("step", 0) < 1 for p in optimizer._stepped()):
+            raise RuntimeError("CapturedStep needs an optimizer that has taken at least one eager step with these parameters "
+                               "(clip_and_step)")
+        self.optimizer, self.params, self.max_norm = optimizer, optimizer._stepped(), float(max_norm)
+        self.plan = optimizer._flat()
+        self.eager = self.plan.table(optimizer.param_groups, optimizer.state)
+        self.runs = list(self.eager.runs)
+        dev = self.plan.device
+        n, r = len(self.eager.sizes), len(self.runs)
+        self.rows_host = torch.empty((n, 5), dtype=torch.int64).pin_memory()
+        self.descs = torch.empty((n, 5), dtype=torch.int64, device=dev)
+        self.ws = torch.empty_like(self.plan.norm_ws)
+        self.dyn_host = [torch.zeros((r, self.WIDTH), dtype=torch.uint8).pin_memory() for _ in range(self.RING)]
+        self.dyn_done = [None] * self.RING
+        self.slot = 0
+        self.dyn = torch.zeros((r, self.WIDTH), dtype=torch.uint8, device=dev)
+        self.order = [p for _, ps, _, _ in self.runs for p in ps]
+        self.norm = None
+
+    def prepare(self):
+        if self.optimizer._plan is not self.plan:
+            raise RuntimeError("the optimizer's state was replaced after the capture")
+        i = self.slot
+        self.slot = (i + 1) % self.RING
+        if self.dyn_done[i] is not None:
+            self.dyn_done[i].synchronize()
+        host = self.dyn_host[i]
+        state = self.optimizer.state
+        for k, (g, ps, _, _) in enumerate(self.runs):
+            steps = {state[p]["step"] for p in ps}
+            if len(steps) != 1:
+                raise RuntimeError("the parameters' step numbers no longer agree: capture the step again")
+            b1, b2 = g["betas"]
+            call("mis_adamw8_step_constants", float(g["lr"]), float(b1), float(b2), float(g["weight_decay"]),
+                 steps.pop() + 1, host[k].data_ptr())
+        self.dyn.copy_(host, non_blocking=True)
+        ev = torch.cuda.Event()
+        ev.record()
+        self.dyn_done[i] = ev
+
+    def launch(self):
+        rows, self.keep = self.plan.rows(self.order)
+        self.rows_host.copy_(torch.tensor(rows, dtype=torch.int64))
+        self.descs.copy_(self.rows_host, non_blocking=True)
+        st = F_._stream()
+        self.norm = self.plan.sqsum(self.eager, st, self.descs, self.ws)
+        for k, (g, _, c0, c1) in enumerate(self.runs):
+            b1, b2 = g["betas"]
+            self.plan.step(self.eager, g, c0, c1, self.max_norm, 0.0, b1, b2, 0.0, 1, self.dyn[k],
+                           self.norm if k == 0 else None, st, self.descs, self.ws)
+        return self.norm
+
+    def advance(self):
+        for p in self.params:
+            self.optimizer.state[p]["step"] += 1
+        torch._C._increment_version(self.params)
+
+
+def captured_step(optimizer, params, max_norm=1.0):
+    """The CapturedStep of this optimizer: prepare(), launch() inside the capture, advance()."""
+    if isinstance(optimizer, AdamW8):
+        return _CapturedStep8(optimizer, params, max_norm)
+    return CapturedStep(optimizer, params, max_norm)
 
 
 class CapturedStep:
