@@ -56,6 +56,286 @@ template <> struct Mma<float> {
 };
 
 // ---------------------------------------------------------------------------------------------------------------
+// Tiles staged straight from memory into LDS (16-byte chunks; sizes, strides and addresses multiples of 16 bytes).
+//
+// A workgroup of WP x WQ waves owns TP x TQ outputs and walks r in steps of 128 bytes (64 bf16, 32 float32).  Two
+// stages of LDS: while the matrix instructions work on one, buffer loads with an LDS destination fill the other; one
+// barrier a stage.  Chunks outside the operand get an offset behind the buffer's end and arrive as zeros.
+//
+// Rows of an operand that is contiguous in r are 128 bytes of LDS; a fragment read takes the same 16-byte chunk of 16
+// rows, so chunk c of row i lies at c ^ ((i / 2) % 8): 16 rows, 16 different 16-byte windows of the 256 bytes of banks.
+// An operand that is contiguous in its rows ("transposed", for the two products of the backward pass) is staged as
+// [r][row].  bf16: ds_read_b64_tr_b16 hands lane i of 16 the column i of a 4 x 16 block; a half-wave reads 8 r-rows of
+// 32 bytes, spread over the banks by the r bits that differ between them.  float32: plain 4-byte reads, 64 bytes wide,
+// four r-rows apart.
+// The loads put an LDS line in the order of the lanes, so the permutation is applied to the addresses they read.
+// ---------------------------------------------------------------------------------------------------------------
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
+constexpr uint32_t OUTSIDE = 0x80000000u;
+constexpr int ROW_BYTES = 128;
+
+// (by value: a __builtin_bit_cast of a vector's element in place takes the first one)
+__device__ __forceinline__ float as_float(uint32_t u) { return __builtin_bit_cast(float, u); }
+__device__ __forceinline__ uint32_t as_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* p) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, 0x7FFFFFF0, 0x00020000);
+}
+
+// 16 bytes per lane from `off` on to consecutive LDS addresses (this wave's from `lds`)
+__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t rs, char* lds, uint32_t off) {
+#ifdef __HIP_DEVICE_COMPILE__          // (the host pass does not know the 16-byte form and drops the kernel without a word)
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)lds, 16, off, 0, 0, 0);
+#endif
+}
+
+// Where the 16-byte chunk `c` of r-row `k` lies in a transposed tile W rows wide.
+template <typename T, int W>
+__device__ __forceinline__ int tr_chunk(int k, int c) {
+  if constexpr (sizeof(T) == 2) {               // by 32-byte units
+    if constexpr (W * 2 >= 256) return c ^ (((k & 3) | (k >> 1 & 4)) << 1);
+    else return c ^ (((k >> 1 & 1) | (k >> 2 & 2)) << 1);
+  } else {
+    return c ^ ((k >> 2 & 3) << 2);             // by 64-byte units
+  }
+}
+
+// One operand's share of a stage: TR false: W rows of 128 bytes; true: 128 / sizeof(T) r-rows of W elements.
+template <typename T, int W, bool TR, int THREADS> struct Stager {
+  static constexpr int BYTES = W * ROW_BYTES, N = BYTES / 16 / THREADS, K = ROW_BYTES / (int)sizeof(T);
+  uint32_t off[N];        // byte offset of this thread's chunks from the operand's first staged element
+  int k[N];               // their first r within the stage
+
+  __device__ __forceinline__ void init(const Operand<T>& o, int row0) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int chunk = i * THREADS + threadIdx.x;
+      if constexpr (!TR) {
+        const int row = chunk >> 3, c = (chunk & 7) ^ (row >> 1 & 7);
+        k[i] = c * (16 / (int)sizeof(T));
+        off[i] = row0 + row < o.rows ? (uint32_t)((int64_t)row * o.s_row * sizeof(T)) + c * 16 : OUTSIDE;
+      } else {
+        constexpr int CR = W * (int)sizeof(T) / 16;           // chunks of an r-row
+        k[i] = chunk / CR;
+        const int c = tr_chunk<T, W>(k[i], chunk % CR);
+        off[i] = row0 + c * (16 / (int)sizeof(T)) < o.rows ? (uint32_t)((int64_t)k[i] * o.s_k * sizeof(T)) + c * 16 : OUTSIDE;
+      }
+    }
+  }
+
+  // `first`: the operand's element (row0, r0 of the stage); left = r elements from there on
+  __device__ __forceinline__ void issue(const T* first, int64_t left, char* lds) const {
+    const __amdgpu_buffer_rsrc_t rs = buffer_at(first);
+    const int wave_base = __builtin_amdgcn_readfirstlane((threadIdx.x & ~63) * 16);
+    const bool whole = left >= K;
+#pragma unroll
+    for (int i = 0; i < N; i++) to_lds(rs, lds + i * THREADS * 16 + wave_base, whole || k[i] < left ? off[i] : OUTSIDE);
+  }
+};
+
+// The fragment of 16 rows from `row` on, half `h` (64 bytes of r) of a stage.  bf16: k = 32 h + 8 g + e; float32:
+// k = 16 h + 4 g + e (e-th instruction), g = lane / 16.
+template <typename T, int W, bool TR>
+__device__ __forceinline__ u32x4 fragment(const char* tile, int row, int h) {
+  const int lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
+  if constexpr (!TR) {
+    const int r = row + j;
+    return *(const u32x4*)(tile + r * ROW_BYTES + (((4 * h + g) ^ (r >> 1 & 7)) << 4));
+  } else if constexpr (sizeof(T) == 2) {
+    union { bf16x4 b[2]; u32x4 u; } f;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int k = 32 * h + 8 * g + 4 * i + (j >> 2), col = row + 4 * (j & 3);
+      f.b[i] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+          (lds_bf16x4*)(tile + k * W * 2 + (tr_chunk<T, W>(k, col >> 3) << 4) + (col & 4) * 2));
+    }
+    return f.u;
+  } else {
+    u32x4 f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int k = 16 * h + 4 * g + e, col = row + j;
+      f[e] = *(const uint32_t*)(tile + k * W * 4 + (tr_chunk<T, W>(k, col >> 2) << 4) + (col & 3) * 4);
+    }
+    return f;
+  }
+}
+
+__device__ __forceinline__ f32x4 multiply(u32x4 a, u32x4 b, f32x4 c, bf16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 multiply(u32x4 a, u32x4 b, f32x4 c, float) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(as_float(a[e]), as_float(b[e]), c, 0, 0, 0);
+  return c;
+}
+
+// 4 (float32) or 8 (bf16) consecutive elements, 16 bytes
+template <typename T> struct Pack {
+  static constexpr int N = 16 / sizeof(T);
+  float v[N];
+  __device__ __forceinline__ void load(const T* p) {
+    union { u32x4 u; T t[N]; } x;
+    x.u = *(const u32x4*)p;
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = to_f32(x.t[i]);
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    union { u32x4 u; T t[N]; } x;
+#pragma unroll
+    for (int i = 0; i < N; i++) x.t[i] = from_f32<T>(v[i]);
+    *(u32x4*)p = x.u;
+  }
+};
+
+// Tile number -> (p tile, q tile, split).  Workgroups go round-robin over the 8 XCDs; each XCD gets a run of
+// neighbouring tiles (its own L2 then holds a few rows of both operands): QGROUP q tiles side by side, p slower.
+constexpr int XCDS = 8, QGROUP = 4;
+struct Grid {
+  int p_tiles, q_tiles, splits;
+  int64_t r_per_split;
+  __host__ __device__ int total() const { return p_tiles * q_tiles * splits; }
+  __host__ __device__ int launch() const { return (total() + XCDS - 1) / XCDS * XCDS; }
+};
+
+template <typename T, int TP, int TQ, int WP, int WQ, bool PTR, bool QTR, int MODE>
+__global__ __launch_bounds__(64 * WP * WQ, 2) void lin_tile_kernel(Operand<T> P, Operand<T> Q, int64_t R, Grid grid,
+                                                                   Epilogue<T> e) {
+  constexpr int THREADS = 64 * WP * WQ, BP = TP / WP / 16, BQ = TQ / WQ / 16, K = ROW_BYTES / (int)sizeof(T);
+  constexpr int STAGE = (TP + TQ) * ROW_BYTES;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+  const int wp = (wave % WP) * (TP / WP), wq = (wave / WP) * (TQ / WQ);
+
+  const int total = grid.total(), per = grid.launch() / XCDS;
+  const int id = ((int)blockIdx.x % XCDS) * per + (int)blockIdx.x / XCDS;
+  if (id >= total) return;
+  const int tiles = grid.p_tiles * grid.q_tiles, split = id / tiles;
+  int t = id - split * tiles;
+  const int group = t / (QGROUP * grid.p_tiles), gq = min(QGROUP, grid.q_tiles - group * QGROUP);
+  t -= group * QGROUP * grid.p_tiles;
+  const int q_tile = group * QGROUP + t % gq, p_tile = t / gq;
+  const int p0 = p_tile * TP, q0 = q_tile * TQ;
+  const int64_t r0 = (int64_t)split * grid.r_per_split, r1 = min(r0 + grid.r_per_split, R);
+
+  Stager<T, TP, PTR, THREADS> sp;
+  Stager<T, TQ, QTR, THREADS> sq;
+  sp.init(P, p0);
+  sq.init(Q, q0);
+  const T* pp = P.p + (int64_t)p0 * P.s_row + r0 * P.s_k;
+  const T* qp = Q.p + (int64_t)q0 * Q.s_row + r0 * Q.s_k;
+
+  f32x4 acc[BP][BQ] = {};
+  if (r0 < r1) {                             // (every load is waited for inside the loop)
+    sp.issue(pp, r1 - r0, lds);
+    sq.issue(qp, r1 - r0, lds + TP * ROW_BYTES);
+  }
+  int cur = 0;
+  for (int64_t r = r0; r < r1; r += K, cur ^= 1) {
+    __syncthreads();                        // this stage has arrived; nobody reads the other one any more
+    if (r + K < r1) {
+      char* next = lds + (cur ^ 1) * STAGE;
+      pp += K * P.s_k;
+      qp += K * Q.s_k;
+      sp.issue(pp, r1 - r - K, next);
+      sq.issue(qp, r1 - r - K, next + TP * ROW_BYTES);
+    }
+    const char* tp = lds + cur * STAGE;
+    const char* tq = tp + TP * ROW_BYTES;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      u32x4 a[BP], b[BQ];
+#pragma unroll
+      for (int i = 0; i < BP; i++) a[i] = fragment<T, TP, PTR>(tp, wp + 16 * i, h);
+#pragma unroll
+      for (int j = 0; j < BQ; j++) b[j] = fragment<T, TQ, QTR>(tq, wq + 16 * j, h);
+#pragma unroll
+      for (int i = 0; i < BP; i++)
+#pragma unroll
+        for (int j = 0; j < BQ; j++) acc[i][j] = multiply(a[i], b[j], acc[i][j], T());
+    }
+  }
+
+  // A lane has p = 4 g + 0..3 of every 16 x 16 block, q = lane % 16.  For 16-byte accesses in bf16 the lanes of two
+  // neighbouring blocks trade halves (v_permlane16_swap): 8 consecutive p of one block each.
+  constexpr bool WIDE = sizeof(T) == 2 && MODE != PARTIAL;
+  constexpr int NV = WIDE ? 8 : 4, PAIRS = WIDE ? BP / 2 : BP;
+  with_act(MODE == FWD || MODE == DZ ? e.act : MIS_ACT_NONE, [&](auto act) {
+    constexpr int ACT = decltype(act)::value;
+#pragma unroll
+    for (int i = 0; i < PAIRS; i++) {
+      const int pl = wp + (WIDE ? 32 * i + 16 * (g & 1) + 8 * (g >> 1) : 16 * i + 4 * g), p = p0 + pl;
+      const bool in_p = p < P.rows;
+      float bias[NV], cs[NV];
+#pragma unroll
+      for (int k = 0; k < NV; k++) {
+        bias[k] = 0.f;
+        cs[k] = 0.f;
+      }
+      if constexpr (MODE == FWD || MODE == DZ)
+        if (e.bias && in_p)
+#pragma unroll
+          for (int k = 0; k < NV; k++) bias[k] = e.bias[p + k];
+#pragma unroll
+      for (int j = 0; j < BQ; j++) {
+        float v[NV];
+        if constexpr (WIDE) {
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const auto s = __builtin_amdgcn_permlane16_swap(as_bits(acc[2 * i][j][k]), as_bits(acc[2 * i + 1][j][k]), false, false);
+            v[k] = as_float(s[0]);
+            v[k + 4] = as_float(s[1]);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; k++) v[k] = acc[i][j][k];
+        }
+        const int64_t q = q0 + wq + 16 * j + (lane & 15);
+        if (!in_p || q >= Q.rows) continue;
+        if constexpr (MODE == PARTIAL) {
+          *(f32x4*)(e.rows + ((int64_t)split * Q.rows + q) * P.rows + p) = f32x4{v[0], v[1], v[2], v[3]};
+        } else {
+          Pack<T> o, x;
+          if constexpr (MODE == FWD)
+            if (e.other) x.load(e.other + q * e.ld + p);
+          if constexpr (MODE == DZ) x.load(e.other + q * e.ld + p);
+#pragma unroll
+          for (int k = 0; k < NV; k++) {
+            o.v[k] = v[k];
+            if constexpr (MODE == FWD) o.v[k] = act_value<ACT>(v[k] + bias[k]) + (e.other ? x.v[k] : 0.f);
+            if constexpr (MODE == DZ) {
+              o.v[k] = x.v[k] * act_slope<ACT>(v[k] + bias[k]);
+              cs[k] += o.v[k];
+            }
+          }
+          o.store(e.out + q * P.rows + p);
+        }
+      }
+      if constexpr (MODE == DZ) {
+        float* colsum = (float*)(lds + 2 * STAGE);           // [WQ][TP]
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+          const float s = row16_sum(cs[k]);
+          if ((lane & 15) == 0) colsum[(wave / WP) * TP + pl + k] = s;
+        }
+      }
+    }
+  });
+  if constexpr (MODE == DZ) {
+    const float* colsum = (const float*)(lds + 2 * STAGE);
+    __syncthreads();
+    for (int c = threadIdx.x; c < TP && p0 + c < P.rows; c += THREADS) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < WQ; w++) s += colsum[w * TP + c];
+      e.rows[(int64_t)q_tile * P.rows + p0 + c] = s;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
 // Any sizes, strides and alignments: 64 x 64 outputs per workgroup, elements staged one by one.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int ANY_T = 64, ANY_K = 32, ANY_PITCH = ANY_K + 8;
@@ -183,10 +463,57 @@ __global__ __launch_bounds__(256) void lin_colsum_kernel(const T* __restrict__ d
 // ---------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------
-template <typename T, int MODE>
-void launch_product(const Operand<T>& P, const Operand<T>& Q, int64_t R, int splits, const Epilogue<T>& e, hipStream_t st) {
-  const int64_t per = ((R + splits - 1) / splits + ANY_K - 1) / ANY_K * ANY_K;
+// Output tile of a product: the q rows that one row of partial sums covers is the kernel's TQ.
+enum Tile { ANY64, T64, T128, T256 };
+int tile_edge(Tile t) { return t == T256 ? 256 : t == T128 ? 128 : 64; }
+
+// Whether the staged kernels take these: everything in 16-byte chunks.
+template <typename T> bool chunked(const Operand<T>& o, int64_t R) {
+  constexpr int V = 16 / sizeof(T);
+  if ((uintptr_t)o.p & 15) return false;
+  if (o.s_k == 1) return R % V == 0 && o.s_row % V == 0 && o.s_row * (int64_t)sizeof(T) * 256 < 0x7FFFFF00;
+  return o.rows % V == 0 && o.s_k % V == 0 && o.s_k * (int64_t)sizeof(T) * 64 < 0x7FFFFF00;
+}
+
+Tile pick_tile(int64_t p, int64_t q, int splits) {
+  if ((int64_t)cdiv(p, 256) * cdiv(q, 256) * splits >= 256) return T256;
+  if ((int64_t)cdiv(p, 128) * cdiv(q, 128) * splits >= 256) return T128;
+  return T64;
+}
+
+template <typename T, int TP, int TQ, int WP, int WQ, bool PTR, bool QTR, int MODE>
+int launch_tile(const Operand<T>& P, const Operand<T>& Q, int64_t R, int splits, int64_t per, const Epilogue<T>& e, hipStream_t st) {
+  constexpr int LDS = 2 * (TP + TQ) * ROW_BYTES + (MODE == DZ ? WQ * TP * 4 : 0);
+  if constexpr (LDS > 65536) {
+    static thread_local bool raised[64] = {};
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev >= 64) return 1;
+    if (!raised[dev]) {
+      if (hipFuncSetAttribute((const void*)lin_tile_kernel<T, TP, TQ, WP, WQ, PTR, QTR, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return 1;
+      raised[dev] = true;
+    }
+  }
+  const Grid g{cdiv(P.rows, TP), cdiv(Q.rows, TQ), splits, per};
+  lin_tile_kernel<T, TP, TQ, WP, WQ, PTR, QTR, MODE><<<g.launch(), 64 * WP * WQ, LDS, st>>>(P, Q, R, g, e);
+  return 0;
+}
+
+template <typename T, bool PTR, bool QTR, int MODE>
+int launch_staged(Tile tile, const Operand<T>& P, const Operand<T>& Q, int64_t R, int splits, int64_t per, const Epilogue<T>& e,
+                  hipStream_t st) {
+  switch (tile) {
+    case T256: return launch_tile<T, 256, 256, 2, 4, PTR, QTR, MODE>(P, Q, R, splits, per, e, st);
+    case T128: return launch_tile<T, 128, 128, 2, 2, PTR, QTR, MODE>(P, Q, R, splits, per, e, st);
+    default: return launch_tile<T, 64, 64, 2, 2, PTR, QTR, MODE>(P, Q, R, splits, per, e, st);
+  }
+}
+
+template <typename T, bool PTR, bool QTR, int MODE>
+int launch_product(Tile tile, const Operand<T>& P, const Operand<T>& Q, int64_t R, int splits, const Epilogue<T>& e, hipStream_t st) {
+  const int64_t per = ((R + splits - 1) / splits + 63) / 64 * 64;
+  if (tile != ANY64) return launch_staged<T, PTR, QTR, MODE>(tile, P, Q, R, splits, per, e, st);
   lin_any_kernel<T, MODE><<<dim3(cdiv(P.rows, ANY_T) * cdiv(Q.rows, ANY_T), splits), 256, 0, st>>>(P, Q, R, per, e);
+  return 0;
 }
 
 // Parts of the long sum of dW: enough workgroups to fill the chip twice, at least 256 rows to a part.
@@ -226,14 +553,24 @@ bool aligned(int dtype, std::initializer_list<const void*> ps) {
 }
 
 template <typename T>
-void forward(const T* x, int64_t ldx, const T* w, const float* bias, const T* r, int64_t ldr, int64_t M, int64_t N, int64_t K,
-             int act, T* y, hipStream_t st) {
-  launch_product<T, FWD>({w, K, 1, (int)N}, {x, ldx, 1, (int)M}, K, 1, {bias, r, ldr, y, nullptr, act}, st);
+Tile tile_for(const Operand<T>& P, const Operand<T>& Q, int64_t R, const Epilogue<T>& e, int splits) {
+  constexpr int V = 16 / sizeof(T);
+  const bool ok = chunked(P, R) && chunked(Q, R) && P.rows % V == 0 && (((uintptr_t)e.other | (uintptr_t)e.out) & 15) == 0 &&
+                  (!e.other || e.ld % V == 0);
+  return ok ? pick_tile(P.rows, Q.rows, splits) : ANY64;
 }
 
 template <typename T>
-void backward(const T* x, int64_t ldx, const T* w, const float* bias, const T* dy, int64_t ldd, int dtype, int64_t M, int64_t N,
-              int64_t K, int act, T* dx, T* dw, float* db, char* ws, hipStream_t st) {
+int forward(const T* x, int64_t ldx, const T* w, const float* bias, const T* r, int64_t ldr, int64_t M, int64_t N, int64_t K,
+            int act, T* y, hipStream_t st) {
+  const Operand<T> P{w, K, 1, (int)N}, Q{x, ldx, 1, (int)M};
+  const Epilogue<T> e{bias, r, ldr, y, nullptr, act};
+  return launch_product<T, false, false, FWD>(tile_for(P, Q, K, e, 1), P, Q, K, 1, e, st);
+}
+
+template <typename T>
+int backward(const T* x, int64_t ldx, const T* w, const float* bias, const T* dy, int64_t ldd, int dtype, int64_t M, int64_t N,
+             int64_t K, int act, T* dx, T* dw, float* db, char* ws, hipStream_t st) {
   const BwdPlan p = bwd_plan(dtype, M, N, K, act);
   T* dz = (T*)ws;
   float* rows = (float*)(ws + p.dz);
@@ -241,24 +578,31 @@ void backward(const T* x, int64_t ldx, const T* w, const float* bias, const T* d
   const T* z = dy;
   int64_t ldz = ldd;
   if (act != MIS_ACT_NONE) {
-    launch_product<T, DZ>({w, K, 1, (int)N}, {x, ldx, 1, (int)M}, K, 1, {bias, dy, ldd, dz, rows, act}, st);
+    const Operand<T> P{w, K, 1, (int)N}, Q{x, ldx, 1, (int)M};
+    const Epilogue<T> e{bias, dy, ldd, dz, rows, act};
+    const Tile tile = tile_for(P, Q, K, e, 1);
+    if (launch_product<T, false, false, DZ>(tile, P, Q, K, 1, e, st)) return 1;
     z = dz;
     ldz = N;
-    if (db) launch_reduce_partials(rows, cdiv(M, ANY_T), (int)N, db, st);
+    if (db) launch_reduce_partials(rows, cdiv(M, tile_edge(tile)), (int)N, db, st);
   } else if (db) {
     lin_colsum_kernel<T><<<dim3(cdiv(M, SUM_ROWS), cdiv(N, 64)), 256, 0, st>>>(dy, ldd, M, (int)N, rows);
     launch_reduce_partials(rows, cdiv(M, SUM_ROWS), (int)N, db, st);
   }
-  if (dx) launch_product<T, STORE>({w, 1, K, (int)K}, {z, ldz, 1, (int)M}, N, 1, {nullptr, nullptr, 0, dx, nullptr, 0}, st);
+  if (dx) {
+    const Operand<T> P{w, 1, K, (int)K}, Q{z, ldz, 1, (int)M};
+    const Epilogue<T> e{nullptr, nullptr, 0, dx, nullptr, 0};
+    if (launch_product<T, true, false, STORE>(tile_for(P, Q, N, e, 1), P, Q, N, 1, e, st)) return 1;
+  }
   if (dw) {
     const Operand<T> P{x, 1, ldx, (int)K}, Q{z, 1, ldz, (int)N};
-    if (p.splits == 1) {
-      launch_product<T, STORE>(P, Q, M, 1, {nullptr, nullptr, 0, dw, nullptr, 0}, st);
-    } else {
-      launch_product<T, PARTIAL>(P, Q, M, p.splits, {nullptr, nullptr, 0, nullptr, part, 0}, st);
-      lin_join_kernel<T><<<ew_grid(N * K, 256), 256, 0, st>>>(part, p.splits, N * K, dw);
-    }
+    const Epilogue<T> e{nullptr, nullptr, 0, dw, part, 0};
+    const Tile tile = tile_for(P, Q, M, e, p.splits);
+    if (p.splits == 1) return launch_product<T, true, true, STORE>(tile, P, Q, M, 1, e, st);
+    if (launch_product<T, true, true, PARTIAL>(tile, P, Q, M, p.splits, e, st)) return 1;
+    lin_join_kernel<T><<<ew_grid(N * K, 256), 256, 0, st>>>(part, p.splits, N * K, dw);
   }
+  return 0;
 }
 
 }  // namespace
@@ -274,10 +618,12 @@ int mis_linear_act_fwd(const void* x, int64_t ldx, const void* w, const float* b
   MIS_REQUIRE(act >= MIS_ACT_NONE && act <= MIS_ACT_GELU, "linear_act_fwd: unknown activation %d", act);
   MIS_REQUIRE(aligned(dtype, {x, w, residual, y}), "linear_act_fwd: misaligned pointer");
   hipStream_t st = (hipStream_t)stream;
+  int rc;
   if (dtype == MIS_BF16)
-    forward((const bf16*)x, ldx, (const bf16*)w, bias, (const bf16*)residual, ldr, M, N, K, act, (bf16*)y, st);
+    rc = forward((const bf16*)x, ldx, (const bf16*)w, bias, (const bf16*)residual, ldr, M, N, K, act, (bf16*)y, st);
   else
-    forward((const float*)x, ldx, (const float*)w, bias, (const float*)residual, ldr, M, N, K, act, (float*)y, st);
+    rc = forward((const float*)x, ldx, (const float*)w, bias, (const float*)residual, ldr, M, N, K, act, (float*)y, st);
+  MIS_REQUIRE(rc == 0, "linear_act_fwd: the device refuses the kernel's shared memory");
   MIS_CHECK_LAUNCH("linear_act_fwd");
   return MIS_OK;
 }
@@ -296,12 +642,14 @@ int mis_linear_act_bwd(const void* x, int64_t ldx, const void* w, const float* b
   MIS_REQUIRE(act >= MIS_ACT_NONE && act <= MIS_ACT_GELU, "linear_act_bwd: unknown activation %d", act);
   MIS_REQUIRE(aligned(dtype, {x, w, dy, dx, dw}) && ((uintptr_t)workspace & 15) == 0, "linear_act_bwd: misaligned pointer");
   hipStream_t st = (hipStream_t)stream;
+  int rc;
   if (dtype == MIS_BF16)
-    backward((const bf16*)x, ldx, (const bf16*)w, bias, (const bf16*)dy, ldd, dtype, M, N, K, act, (bf16*)dx, (bf16*)dw, db,
+    rc = backward((const bf16*)x, ldx, (const bf16*)w, bias, (const bf16*)dy, ldd, dtype, M, N, K, act, (bf16*)dx, (bf16*)dw, db,
              (char*)workspace, st);
   else
-    backward((const float*)x, ldx, (const float*)w, bias, (const float*)dy, ldd, dtype, M, N, K, act, (float*)dx, (float*)dw, db,
+    rc = backward((const float*)x, ldx, (const float*)w, bias, (const float*)dy, ldd, dtype, M, N, K, act, (float*)dx, (float*)dw, db,
              (char*)workspace, st);
+  MIS_REQUIRE(rc == 0, "linear_act_bwd: the device refuses the kernel's shared memory");
   MIS_CHECK_LAUNCH("linear_act_bwd");
   return MIS_OK;
 }
