@@ -11,6 +11,8 @@ torch's own `clip_grad_norm_` + `optimizer.step()` unchanged.
 `AdamW8` is the same update with both moments in 8 bits (2.02 bytes of state per parameter instead of 8);
 `clip_and_step` and `CapturedStep` take it as they take torch's AdamW.
 """
+import operator
+
 import torch
 
 from .. import functional as F_
@@ -127,11 +129,13 @@ def clip_and_step(optimizer, params, max_norm=1.0):
     params = [p for p in params]
     F_.flush_wgrad_reduces()       # (a no-op after a finished backward pass)
     if isinstance(optimizer, AdamW8):
-        if {id(p) for p in params if p.grad is not None} != {id(p) for p in optimizer._stepped()}:
+        stepped, given = optimizer._stepped(), [p for p in params if p.grad is not None]
+        same = len(stepped) == len(given) and all(map(operator.is_, stepped, given))
+        if not same and {id(p) for p in given} != {id(p) for p in stepped}:
             norm = torch.nn.utils.clip_grad_norm_(params, max_norm=max_norm)   # a norm over other tensors than are stepped
             optimizer.step()
             return norm
-        return optimizer._launch(float(max_norm))
+        return optimizer._launch(float(max_norm), stepped)
     fast = _fast_path(optimizer, params)
     if fast is not None:
         return _launch(optimizer, fast, max_norm)
@@ -314,7 +318,7 @@ class AdamW8(torch.optim.Optimizer):
         """The flat moment buffers, laid out over all parameters; state[p] holds views of them."""
         params = [p for g in self.param_groups for p in g["params"]]
         plan = self._plan
-        if plan is not None and plan.matches(params, self.state):
+        if plan is not None and plan.matches(params):
             return plan
         devs = {p.device for p in params}
         if len(devs) != 1 or next(iter(devs)).type != "cuda":
@@ -327,6 +331,8 @@ class AdamW8(torch.optim.Optimizer):
                 s[k] = buf[b0 * w:b1 * w]
                 if k in old:
                     s[k].copy_(old[k])
+                    if w == BLOCK8:
+                        s[k][p.numel():].zero_()
             s["step"] = int(old.get("step", 0))
         return plan
 
@@ -338,10 +344,10 @@ class AdamW8(torch.optim.Optimizer):
         b0, b1 = (0, plan.blocks) if p is None else plan.spans[[id(q) for q in plan.params].index(id(p))]
         out = [torch.empty((b1 - b0) * BLOCK8, dtype=torch.float32, device=dev) for _ in range(2)]
         if b1 > b0:
-            m, ms, v, vs = plan.buffers
+            m, ms, v, vs = (b.data_ptr() for b in plan.buffers)
             with F_._on_device_of(out[0]):
-                call("mis_adamw8_moments", m[b0 * BLOCK8:].data_ptr(), ms[b0:].data_ptr(), v[b0 * BLOCK8:].data_ptr(),
-                     vs[b0:].data_ptr(), b1 - b0, out[0].data_ptr(), out[1].data_ptr(), F_._stream())
+                call("mis_adamw8_moments", m + b0 * BLOCK8, ms + b0, v + b0 * BLOCK8, vs + b0, b1 - b0, out[0].data_ptr(),
+                     out[1].data_ptr(), F_._stream())
         if p is None:
             return out[0], out[1]
         return tuple(torch.as_strided(t, p.shape, p.stride()).clone(memory_format=torch.preserve_format) for t in out)
@@ -352,29 +358,23 @@ class AdamW8(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        self._launch(None)
+        self._launch(None, self._stepped())
         return loss
 
-    @torch.no_grad()
-    def _launch(self, max_norm):
-        """One step; max_norm None: no norm is formed.  Returns the total gradient norm otherwise."""
-        params = self._stepped()
+    def _launch(self, max_norm, params):
+        """One step of `params`, those with a gradient; max_norm None: no norm is formed.  Returns the total gradient norm
+        otherwise."""
         if not params:
             return torch.zeros(()) if max_norm is not None else None
         if params[0].is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("an AdamW8 step cannot be captured as it is (its step number would be frozen): use "
                                "CapturedStep or GraphedTrainStep")
-        plan = self._flat()
-        table = plan.table(self.param_groups, self.state)
-        with F_._on_device_of(plan.buffers[0]):
-            st = F_._stream()
-            norm = plan.sqsum(table, st) if max_norm is not None else None
-            for k, (g, ps, c0, c1) in enumerate(table.runs):
-                b1, b2 = g["betas"]
-                plan.step(table, g, c0, c1, max_norm, float(g["lr"]), b1, b2, float(g["weight_decay"]),
-                          self.state[ps[0]]["step"] + 1, None, norm if k == 0 else None, st)
-        for p in params:
-            self.state[p]["step"] += 1
+        table = self._flat().table(self.param_groups, self.state, params)
+        norm = table.launch(max_norm)
+        for states in table.states:
+            k = states[0]["step"] + 1
+            for s in states:
+                s["step"] = k
         torch._C._increment_version(params)
         return norm
 
@@ -393,78 +393,113 @@ class _Plan8:
         self.blocks = at
         self.buffers = [torch.zeros(max(at, 1) * w, dtype=torch.uint8, device=device) for w in (BLOCK8, 1, BLOCK8, 1)]
         self.norm_ws = torch.empty(query("mis_adamw8_workspace_bytes"), dtype=torch.uint8, device=device)
-        self.tables = {}
+        self.tables = []
 
-    def matches(self, params, state):
-        if len(params) != len(self.params) or any(a is not b for a, b in zip(params, self.params)):
-            return False
-        base = self.buffers[0].data_ptr()
-        return all("exp_avg" in state[p] and state[p]["exp_avg"].data_ptr() == base + b0 * BLOCK8 and p.device == self.device
-                   for p, (b0, b1) in zip(params, self.spans) if b1 > b0)
+    def matches(self, params):
+        return len(params) == len(self.params) and all(map(operator.is_, params, self.params))
 
-    def rows(self, params):
-        """Pointer rows; a gradient in another memory order than its parameter is copied into the parameter's."""
-        span = {id(p): s for p, s in zip(self.params, self.spans)}
-        rows, keep = [], []
-        for p in params:
-            g = p.grad
-            if g.is_sparse or g.dtype != p.dtype or g.device != p.device:
-                raise RuntimeError(f"AdamW8 needs dense gradients of the parameter's type and device, got {g.dtype} "
-                                   f"{g.layout} on {g.device}")
-            if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
-                g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
-                keep.append(g)
-            rows.append((p.data_ptr(), g.data_ptr(), span[id(p)][0] * BLOCK8, p.numel(), F_._DT[p.dtype]))
-        return rows, keep
+    def table(self, groups, state, params):
+        """The launch tables for `params`, the parameters that have a gradient now."""
+        for t in self.tables:
+            if t.serves(params):
+                break
+        else:
+            if len(self.tables) >= 4:             # (a few patterns of missing gradients at most; not a growing cache)
+                self.tables.clear()
+            t = _Table8(self, groups, state, params)
+            self.tables.append(t)
+        t.refresh()
+        return t
 
-    def table(self, groups, state):
-        """The launch tables for the parameters that have a gradient now: pointer rows, and runs (group, parameters,
-        first chunk, end chunk) of one group and one step number, each of them a launch."""
-        runs, order = [], []
+
+class _Table8:
+    """The device tables for one set of parameters with gradients: pointer rows, chunk prefix, and the runs of one group
+    and one step number, each of them a launch."""
+
+    def __init__(self, plan, groups, state, params):
+        self.plan, self.params = plan, params
+        self.runs, self.states, self.order = [], [], []       # (group, first chunk, end chunk); their states; flat
+        prefix, idle = [0], []
+        stepped = {id(p) for p in params}
         for g in groups:
             by_step = {}
             for p in g["params"]:
-                if p.grad is not None and p.numel():
-                    by_step.setdefault(state[p]["step"], []).append(p)
+                if id(p) in stepped:
+                    if p.numel():
+                        by_step.setdefault(state[p]["step"], []).append(p)
+                    else:
+                        idle.append(state[p])
             for ps in by_step.values():
-                runs.append((g, ps))
-                order += ps
-        rows, keep = self.rows(order)
-        sizes = tuple(r[3] for r in rows)
-        t = self.tables.get(sizes)
-        if t is None:
-            if len(self.tables) >= 8:             # (a few patterns of missing gradients at most; not a growing cache)
-                self.tables.clear()
-            prefix = [0]
-            for n in sizes:
-                prefix.append(prefix[-1] + (n + CHUNK - 1) // CHUNK)
-            t = self.tables[sizes] = _Plan(sizes, None, prefix, self.device)
-        if order and t.rows != rows:
-            t.upload(rows)
-        t.keep = keep                              # (alive until the next step's table replaces them)
-        t.runs, c = [], 0
-        for g, ps in runs:
-            c0 = c
-            for p in ps:
-                c += (p.numel() + CHUNK - 1) // CHUNK
-            t.runs.append((g, ps, c0, c))
-        return t
+                c0 = prefix[-1]
+                for p in ps:
+                    prefix.append(prefix[-1] + (p.numel() + CHUNK - 1) // CHUNK)
+                self.runs.append((g, c0, prefix[-1]))
+                self.states.append([state[p] for p in ps])
+                self.order += ps
+        self.states += [[s] for s in idle]                     # (empty tensors count steps and nothing else)
+        span = {id(p): s for p, s in zip(plan.params, plan.spans)}
+        self.fixed = [(span[id(p)][0] * BLOCK8, p.numel(), F_._DT[p.dtype]) for p in self.order]
+        self.plain = [p.is_contiguous() for p in self.order]
+        self.pointers = self.keep = None
+        self.plan_dev = _Plan([f[1] for f in self.fixed], None, prefix, plan.device) if self.order else None
 
-    def sqsum(self, table, st, descs=None, ws=None):
-        ws = self.norm_ws if ws is None else ws
-        if not table.n_chunks:
-            return torch.zeros((), dtype=torch.float32, device=self.device)
-        call("mis_adamw8_sqsum", (table.descs if descs is None else descs).data_ptr(), table.prefix.data_ptr(),
-             len(table.sizes), table.n_chunks, ws.data_ptr(), st)
-        return torch.empty((), dtype=torch.float32, device=self.device)
+    def serves(self, params):
+        """Whether these are its parameters, and every run still has one step number."""
+        if len(params) != len(self.params) or not all(map(operator.is_, params, self.params)):
+            return False
+        for states in self.states:
+            k = states[0]["step"]
+            if not all([s["step"] == k for s in states]):
+                return False
+        return True
 
-    def step(self, table, g, c0, c1, max_norm, lr, b1, b2, wd, step, dyn, norm, st, descs=None, ws=None):
-        ws = self.norm_ws if ws is None else ws
-        m, ms, v, vs = self.buffers
-        call("mis_adamw8_step", (table.descs if descs is None else descs).data_ptr(), table.prefix.data_ptr(),
-             len(table.sizes), c0, c1, table.n_chunks, m.data_ptr(), ms.data_ptr(), v.data_ptr(), vs.data_ptr(),
-             ws.data_ptr() if max_norm is not None else None, 0.0 if max_norm is None else max_norm, lr, float(b1), float(b2),
-             float(g["eps"]), wd, step, g["seed"], F_._p(dyn), F_._p(norm), st)
+    def addresses(self):
+        """[parameter, gradient, parameter, ...] pointers; a gradient in another memory order than its parameter is copied
+        into the parameter's."""
+        dev, out, keep = self.plan.device, [], []
+        for p, plain in zip(self.order, self.plain):
+            g = p.grad
+            if g.dtype is not p.dtype or g.layout is not torch.strided or g.device != dev or p.device != dev:
+                raise RuntimeError(f"AdamW8 needs dense gradients of the parameter's type and device, got {g.dtype} "
+                                   f"{g.layout} on {g.device} for {p.dtype} on {p.device}")
+            if not (plain and g.is_contiguous()) and g.stride() != p.stride():
+                g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g.detach())
+                keep.append(g)
+            out += (p.data_ptr(), g.data_ptr())
+        return out, keep
+
+    def rows(self, pointers):
+        return [(pointers[2 * i], pointers[2 * i + 1], *f) for i, f in enumerate(self.fixed)]
+
+    def refresh(self):
+        if not self.order:
+            return
+        with F_._on_device_of(self.plan.norm_ws):
+            pointers, self.keep = self.addresses()              # (kept until the next step's replace them)
+            if pointers != self.pointers:
+                self.plan_dev.upload(self.rows(pointers))
+                self.pointers = pointers
+
+    def launch(self, max_norm, descs=None, norm_ws=None, dyn=None):
+        """The launches of a step on the current stream.  dyn: per run, the device constants of a captured step."""
+        plan = self.plan
+        if not self.order:
+            return torch.zeros((), dtype=torch.float32, device=plan.device) if max_norm is not None else None
+        with F_._on_device_of(plan.norm_ws):
+            st, t = F_._stream(), self.plan_dev
+            d, prefix, n = (t.descs if descs is None else descs).data_ptr(), t.prefix.data_ptr(), len(self.order)
+            buffers = [b.data_ptr() for b in plan.buffers]
+            norm = ws = None
+            if max_norm is not None:
+                ws = (plan.norm_ws if norm_ws is None else norm_ws).data_ptr()
+                call("mis_adamw8_sqsum", d, prefix, n, t.n_chunks, ws, st)
+                norm = torch.empty((), dtype=torch.float32, device=plan.device)
+            for k, (g, c0, c1) in enumerate(self.runs):
+                b1, b2 = g["betas"]
+                call("mis_adamw8_step", d, prefix, n, c0, c1, t.n_chunks, *buffers, ws, max_norm or 0.0, float(g["lr"]),
+                     float(b1), float(b2), float(g["eps"]), float(g["weight_decay"]), self.states[k][0]["step"] + 1, g["seed"],
+                     None if dyn is None else dyn[k].data_ptr(), norm.data_ptr() if norm is not None and k == 0 else None, st)
+        return norm
 
 
 class _CapturedStep8:
@@ -473,18 +508,15 @@ class _CapturedStep8:
     RING, WIDTH = 8, 32           # bytes per run's constants (20 used)
 
     def __init__(self, optimizer, params, max_norm):
-        params = list(params)
-        if {id(p) for p in params if p.grad is not None} != {id(p) for p in optimizer._stepped()} or not params:
+        self.optimizer, self.params, self.max_norm = optimizer, optimizer._stepped(), float(max_norm)
+        if {id(p) for p in params if p.grad is not None} != {id(p) for p in self.params} or not self.params:
             raise RuntimeError("CapturedStep needs the gradients of exactly the tensors that the optimizer steps")
-        if any(optimizer.state[p].get("step", 0) < 1 for p in optimizer._stepped()):
+        if any(optimizer.state[p].get("step", 0) < 1 for p in self.params):
             raise RuntimeError("CapturedStep needs an optimizer that has taken at least one eager step with these parameters "
                                "(clip_and_step)")
-        self.optimizer, self.params, self.max_norm = optimizer, optimizer._stepped(), float(max_norm)
         self.plan = optimizer._flat()
-        self.eager = self.plan.table(optimizer.param_groups, optimizer.state)
-        self.runs = list(self.eager.runs)
-        dev = self.plan.device
-        n, r = len(self.eager.sizes), len(self.runs)
+        self.table = _Table8(self.plan, optimizer.param_groups, optimizer.state, self.params)
+        dev, n, r = self.plan.device, len(self.table.order), max(len(self.table.runs), 1)
         self.rows_host = torch.empty((n, 5), dtype=torch.int64).pin_memory()
         self.descs = torch.empty((n, 5), dtype=torch.int64, device=dev)
         self.ws = torch.empty_like(self.plan.norm_ws)
@@ -492,45 +524,38 @@ class _CapturedStep8:
         self.dyn_done = [None] * self.RING
         self.slot = 0
         self.dyn = torch.zeros((r, self.WIDTH), dtype=torch.uint8, device=dev)
-        self.order = [p for _, ps, _, _ in self.runs for p in ps]
         self.norm = None
 
     def prepare(self):
         if self.optimizer._plan is not self.plan:
             raise RuntimeError("the optimizer's state was replaced after the capture")
+        if not self.table.serves(self.params):
+            raise RuntimeError("the parameters' step numbers no longer agree: capture the step again")
         i = self.slot
         self.slot = (i + 1) % self.RING
         if self.dyn_done[i] is not None:
             self.dyn_done[i].synchronize()
         host = self.dyn_host[i]
-        state = self.optimizer.state
-        for k, (g, ps, _, _) in enumerate(self.runs):
-            steps = {state[p]["step"] for p in ps}
-            if len(steps) != 1:
-                raise RuntimeError("the parameters' step numbers no longer agree: capture the step again")
+        for k, (g, _, _) in enumerate(self.table.runs):
             b1, b2 = g["betas"]
             call("mis_adamw8_step_constants", float(g["lr"]), float(b1), float(b2), float(g["weight_decay"]),
-                 steps.pop() + 1, host[k].data_ptr())
+                 self.table.states[k][0]["step"] + 1, host[k].data_ptr())
         self.dyn.copy_(host, non_blocking=True)
         ev = torch.cuda.Event()
         ev.record()
         self.dyn_done[i] = ev
 
     def launch(self):
-        rows, self.keep = self.plan.rows(self.order)
-        self.rows_host.copy_(torch.tensor(rows, dtype=torch.int64))
+        pointers, self.keep = self.table.addresses()
+        self.rows_host.copy_(torch.tensor(self.table.rows(pointers), dtype=torch.int64))
         self.descs.copy_(self.rows_host, non_blocking=True)
-        st = F_._stream()
-        self.norm = self.plan.sqsum(self.eager, st, self.descs, self.ws)
-        for k, (g, _, c0, c1) in enumerate(self.runs):
-            b1, b2 = g["betas"]
-            self.plan.step(self.eager, g, c0, c1, self.max_norm, 0.0, b1, b2, 0.0, 1, self.dyn[k],
-                           self.norm if k == 0 else None, st, self.descs, self.ws)
+        self.norm = self.table.launch(self.max_norm, self.descs, self.ws, self.dyn)
         return self.norm
 
     def advance(self):
-        for p in self.params:
-            self.optimizer.state[p]["step"] += 1
+        for states in self.table.states:
+            for s in states:
+                s["step"] += 1
         torch._C._increment_version(self.params)
 
 
