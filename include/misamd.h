@@ -651,8 +651,9 @@ int mis_group_norm_act_bwd(const void* x, const void* dy, int dtype, int B, int6
 /*   dz = dy act'(u);  dx = dz W;  dw = dz^T x;  db = sum over rows of dz           */
 /* (dr is dy).  dx, dw dense in the element type, db float32; each may be NULL.     */
 /* dy has row stride ldd.  M < 2^30, N and K <= 2^20.                               */
+size_t mis_linear_act_fwd_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
 int mis_linear_act_fwd(const void* x, int64_t ldx, const void* w, const float* bias, const void* residual, int64_t ldr, int dtype,
-                       int64_t M, int64_t N, int64_t K, int act, void* y, mis_stream_t stream);
+                       int64_t M, int64_t N, int64_t K, int act, void* y, void* workspace, mis_stream_t stream);
 size_t mis_linear_act_bwd_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K, int act);
 int mis_linear_act_bwd(const void* x, int64_t ldx, const void* w, const float* bias, const void* dy, int64_t ldd, int dtype,
                        int64_t M, int64_t N, int64_t K, int act, void* dx, void* dw, float* db, void* workspace,

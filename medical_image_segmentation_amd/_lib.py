@@ -110,7 +110,8 @@ PROTOTYPES = {
     "mis_group_norm_act_fwd": (_i, [_vp, _i, _i, _i64, _i, _i, _vp, _vp, _d, _i, _vp, _vp, _vp, _vp]),
     "mis_group_norm_act_bwd_workspace_bytes": (_sz, [_i, _i, _i64, _i, _i]),
     "mis_group_norm_act_bwd": (_i, [_vp, _vp, _i, _i, _i64, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp]),
-    "mis_linear_act_fwd": (_i, [_vp, _i64, _vp, _vp, _vp, _i64, _i, _i64, _i64, _i64, _i, _vp, _vp]),
+    "mis_linear_act_fwd_workspace_bytes": (_sz, [_i, _i64, _i64, _i64]),
+    "mis_linear_act_fwd": (_i, [_vp, _i64, _vp, _vp, _vp, _i64, _i, _i64, _i64, _i64, _i, _vp, _vp, _vp]),
     "mis_linear_act_bwd_workspace_bytes": (_sz, [_i, _i64, _i64, _i64, _i]),
     "mis_linear_act_bwd": (_i, [_vp, _i64, _vp, _vp, _vp, _i64, _i, _i64, _i64, _i64, _i, _vp, _vp, _vp, _vp, _vp]),
     "mis_adamw8_workspace_bytes": (_sz, []),

@@ -66,43 +66,55 @@ __device__ __forceinline__ Slab slab_of(const Shape& s, int i) {
   return r;
 }
 
-// sums[b][chunk*parts + part][g] = (sum x, sum x*x) over the chunk's pixels and the slab's channels of g
-template <typename T, int V>
+// sums[b][chunk*parts + part][g] = (sum x, sum x*x) over the chunk's pixels and the slab's channels of g.
+// U: channels of a vector that are sure to share a group (a power of two that divides V and the group), so a thread holds
+// V/U pairs of sums and not V: few enough registers for eight waves to a SIMD, which the stream of loads needs.
+template <typename T, int V, int U>
 __global__ __launch_bounds__(GN_THREADS) void gn_sums_kernel(const T* __restrict__ x, Shape s, double2* __restrict__ sums) {
+  constexpr int N = V / U;
   extern __shared__ __attribute__((aligned(16))) char gn_lds[];
-  double2* red = (double2*)gn_lds;                       // [PR][CV*V]
+  double2* red = (double2*)gn_lds;                       // [PR][CV*N]
   const int b = blockIdx.z, tid = threadIdx.x;
   const Slab sl = slab_of(s, blockIdx.y);
   const int cv = tid % s.CV, pr = tid / s.CV;
   const int64_t p0 = (int64_t)blockIdx.x * s.ppc, p1 = min(p0 + s.ppc, s.HW);
   const bool on = pr < s.PR && cv * V < sl.nc;
-  double a1[V], a2[V];
-#pragma unroll
-  for (int k = 0; k < V; k++) a1[k] = a2[k] = 0.0;
   if (on) {
+    double a1[N], a2[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) a1[k] = a2[k] = 0.0;
     const T* xp = x + (int64_t)b * s.HW * s.C + sl.c0 + cv * V;
-#pragma unroll 4
-    for (int64_t p = p0 + pr; p < p1; p += s.PR) {
-      Vec<T, V> v;
-      v.u = *(const typename Bits<T, V>::type*)(xp + p * s.C);
+    auto add = [&](const Vec<T, V>& v) {
 #pragma unroll
       for (int k = 0; k < V; k++) {
         const double d = (double)to_f32(v.t[k]);
-        a1[k] += d;
-        a2[k] = fma(d, d, a2[k]);
+        a1[k / U] += d;
+        a2[k / U] = fma(d, d, a2[k / U]);
       }
+    };
+    int64_t p = p0 + pr;
+    for (; p + 3 * s.PR < p1; p += 4 * s.PR) {           // four loads ahead of the sums
+      Vec<T, V> v[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[i].u = *(const typename Bits<T, V>::type*)(xp + (p + i * s.PR) * s.C);
+#pragma unroll
+      for (int i = 0; i < 4; i++) add(v[i]);
+    }
+    for (; p < p1; p += s.PR) {
+      Vec<T, V> v;
+      v.u = *(const typename Bits<T, V>::type*)(xp + p * s.C);
+      add(v);
     }
 #pragma unroll
-    for (int k = 0; k < V; k++) red[(pr * s.CV + cv) * V + k] = make_double2(a1[k], a2[k]);
+    for (int k = 0; k < N; k++) red[(pr * s.CV + cv) * N + k] = make_double2(a1[k], a2[k]);
   }
   __syncthreads();
-  const int W = s.CV * V;
+  const int W = s.CV * N, nc = sl.nc / U;
   int n = s.PR;
   while (n > 1) {                                        // pixel rows: halves onto halves
     const int h = (n + 1) >> 1;
     for (int i = tid; i < (n - h) * W; i += GN_THREADS) {
-      const int r = i / W, c = i - r * W;
-      if (c < sl.nc) {
+      if (i % W < nc) {
         red[i].x += red[i + h * W].x;
         red[i].y += red[i + h * W].y;
       }
@@ -112,7 +124,7 @@ __global__ __launch_bounds__(GN_THREADS) void gn_sums_kernel(const T* __restrict
   }
   const int part = s.parts == 1 ? 0 : blockIdx.y % s.parts;
   double2* out = sums + ((int64_t)b * s.chunks * s.parts + (int64_t)blockIdx.x * s.parts + part) * s.G;
-  const int gc = s.parts == 1 ? s.Cg : sl.nc;
+  const int gc = (s.parts == 1 ? s.Cg : sl.nc) / U;
   for (int g = tid; g < sl.ng; g += GN_THREADS) {
     double t1 = 0.0, t2 = 0.0;
     for (int c = 0; c < gc; c++) {
@@ -266,49 +278,68 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_sums_kernel(const T* __rest
   }
 }
 
-// chan[b][2][C] = sums over the chunks; dbeta, dgamma = sums over the samples.  Block (32 channels, 8 row lanes).
-__global__ __launch_bounds__(256) void gn_bwd_channels_kernel(const float* __restrict__ rows, int B, int chunks, int C,
-                                                              float* __restrict__ chan, float* __restrict__ dgamma,
-                                                              float* __restrict__ dbeta) {
+// chan[b][2][C] = sums over the chunks; block = 32 channels of one sample, 8 row lanes
+__global__ __launch_bounds__(256) void gn_bwd_channels_kernel(const float* __restrict__ rows, int chunks, int C,
+                                                              float* __restrict__ chan) {
   __shared__ double2 red[8][33];
-  const int lane = threadIdx.x & 31, r = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-  double s1 = 0.0, s2 = 0.0;
-  for (int b = 0; b < B; b++) {
-    double t1 = 0.0, t2 = 0.0;
-    if (c < C) {
-      const float* p = rows + (int64_t)b * chunks * 2 * C + c;
-      for (int i = r; i < chunks; i += 8) {
-        t1 += (double)p[(int64_t)i * 2 * C];
-        t2 += (double)p[(int64_t)i * 2 * C + C];
-      }
+  const int lane = threadIdx.x & 31, r = threadIdx.x >> 5, c = blockIdx.x * 32 + lane, b = blockIdx.y;
+  double t1 = 0.0, t2 = 0.0;
+  if (c < C) {
+    const float* p = rows + (int64_t)b * chunks * 2 * C + c;
+#pragma unroll 4
+    for (int i = r; i < chunks; i += 8) {
+      t1 += (double)p[(int64_t)i * 2 * C];
+      t2 += (double)p[(int64_t)i * 2 * C + C];
     }
-    red[r][lane] = make_double2(t1, t2);
-    __syncthreads();
-    if (r == 0 && c < C) {
-      for (int i = 1; i < 8; i++) {
-        t1 += red[i][lane].x;
-        t2 += red[i][lane].y;
-      }
-      chan[(int64_t)b * 2 * C + c] = (float)t1;
-      chan[(int64_t)b * 2 * C + C + c] = (float)t2;
-      s1 += t1;
-      s2 += t2;
-    }
-    __syncthreads();
   }
+  red[r][lane] = make_double2(t1, t2);
+  __syncthreads();
   if (r == 0 && c < C) {
-    if (dbeta) dbeta[c] = (float)s1;
-    if (dgamma) dgamma[c] = (float)s2;
+    for (int i = 1; i < 8; i++) {
+      t1 += red[i][lane].x;
+      t2 += red[i][lane].y;
+    }
+    chan[(int64_t)b * 2 * C + c] = (float)t1;
+    chan[(int64_t)b * 2 * C + C + c] = (float)t2;
   }
 }
 
-// coef[b][g] = (m1, m2): one wave per (b, g)
-__global__ __launch_bounds__(64) void gn_bwd_coef_kernel(const float* __restrict__ chan, const float* __restrict__ gamma, int C,
-                                                         int Cg, int G, double count, float2* __restrict__ coef) {
-  const int g = blockIdx.x, b = blockIdx.y;
+// The first blocks: dbeta, dgamma = sums of chan over the samples, 64 channels x 4 sample lanes a block.
+// The others (launched only if dx is wanted): coef[b][g] = (m1, m2), one wave per (b, g).
+__global__ __launch_bounds__(256) void gn_bwd_finish_kernel(const float* __restrict__ chan, const float* __restrict__ gamma, int B,
+                                                            int C, int Cg, int G, double count, int channel_blocks,
+                                                            float2* __restrict__ coef, float* __restrict__ dgamma,
+                                                            float* __restrict__ dbeta) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if ((int)blockIdx.x < channel_blocks) {
+    __shared__ double2 red[4][64];
+    const int c = blockIdx.x * 64 + lane;
+    double s1 = 0.0, s2 = 0.0;
+    if (c < C) {
+#pragma unroll 4
+      for (int b = wave; b < B; b += 4) {
+        s1 += (double)chan[(int64_t)b * 2 * C + c];
+        s2 += (double)chan[(int64_t)b * 2 * C + C + c];
+      }
+    }
+    red[wave][lane] = make_double2(s1, s2);
+    __syncthreads();
+    if (wave == 0 && c < C) {
+      for (int w = 1; w < 4; w++) {
+        s1 += red[w][lane].x;
+        s2 += red[w][lane].y;
+      }
+      if (dbeta) dbeta[c] = (float)s1;
+      if (dgamma) dgamma[c] = (float)s2;
+    }
+    return;
+  }
+  const int64_t bg = ((int64_t)blockIdx.x - channel_blocks) * 4 + wave;
+  if (bg >= (int64_t)B * G) return;
+  const int b = (int)(bg / G), g = (int)(bg - (int64_t)b * G);
   const float* p = chan + (int64_t)b * 2 * C + (int64_t)g * Cg;
   double t1 = 0.0, t2 = 0.0;
-  for (int c = threadIdx.x; c < Cg; c += 64) {
+  for (int c = lane; c < Cg; c += 64) {
     const double w = gamma ? (double)gamma[g * Cg + c] : 1.0;
     t1 += w * (double)p[c];
     t2 += w * (double)p[C + c];
@@ -318,7 +349,7 @@ __global__ __launch_bounds__(64) void gn_bwd_coef_kernel(const float* __restrict
     t1 += __shfl_xor(t1, o, WAVE);
     t2 += __shfl_xor(t2, o, WAVE);
   }
-  if (threadIdx.x == 0) coef[(int64_t)b * G + g] = make_float2((float)(t1 / count), (float)(t2 / count));
+  if (lane == 0) coef[bg] = make_float2((float)(t1 / count), (float)(t2 / count));
 }
 
 template <typename T, int V, int ACT>
@@ -361,6 +392,214 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_dx_kernel(const T* __restri
 }
 
 // ---------------------------------------------------------------------------------------------------------------
+// One workgroup holds a slab of whole groups of one sample in registers (RES_THREADS threads, NV vectors each): x (and
+// dy) are read once, the forward is one launch.  Vectors never straddle a group here.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int RES_THREADS = 512, RES_WAVES = RES_THREADS / 64;
+
+// Sum over all threads of a group of the two values per thread; valid in red_out[group] after the barrier.
+// Thread tid holds channel vector tid % CV of pixel row tid / CV; a group is GV neighbouring vectors.
+__device__ __forceinline__ void group_sums(double s1, double s2, int CV, int GV, int ng, int PR, double2* red, double2* out) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  red[tid] = make_double2(s1, s2);
+  __syncthreads();
+  const int n = PR * GV;
+  for (int g = wave; g < ng; g += RES_WAVES) {
+    double t1 = 0.0, t2 = 0.0;
+    for (int e = lane; e < n; e += 64) {
+      const int r = e / GV;
+      const double2 v = red[r * CV + g * GV + (e - r * GV)];
+      t1 += v.x;
+      t2 += v.y;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      t1 += __shfl_xor(t1, o, WAVE);
+      t2 += __shfl_xor(t2, o, WAVE);
+    }
+    if (lane == 0) out[g] = make_double2(t1, t2);
+  }
+  __syncthreads();
+}
+
+// (sample, slab) of a workgroup: the slabs of a sample, which share its memory lines, run on one XCD (workgroups are dealt
+// to the 8 XCDs in turn).
+__device__ __forceinline__ bool resident_place(const Shape& s, int B, int& b, int& slab) {
+  const int total = B * s.slabs, per = ((int)gridDim.x + 7) / 8, id = ((int)blockIdx.x % 8) * per + (int)blockIdx.x / 8;
+  b = id / s.slabs;
+  slab = id - b * s.slabs;
+  return id < total;
+}
+
+template <typename T, int V, int NV, int ACT>
+__global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_kernel(const T* __restrict__ x, Shape s, int B, double eps,
+                                                                     const float* __restrict__ gamma,
+                                                                     const float* __restrict__ beta, T* __restrict__ y,
+                                                                     double2* __restrict__ stats) {
+  __shared__ double2 red[RES_THREADS], grp[RES_THREADS];
+  int b, slab;
+  if (!resident_place(s, B, b, slab)) return;
+  const Slab sl = slab_of(s, slab);
+  const int tid = threadIdx.x, cv = tid % s.CV, pr = tid / s.CV, HW = (int)s.HW;
+  const bool on = pr < s.PR && cv * V < sl.nc;
+  const int64_t base = (int64_t)b * s.HW * s.C + sl.c0 + (on ? cv * V : 0);
+  Vec<T, V> v[NV];
+#pragma unroll
+  for (int i = 0; i < NV; i++) {
+    const int p = min(pr + i * s.PR, HW - 1);
+    v[i].u = *(const typename Bits<T, V>::type*)(x + base + (int64_t)p * s.C);
+  }
+  double s1 = 0.0, s2 = 0.0;
+  if (on) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      if (pr + i * s.PR < HW) {
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+          const double d = (double)to_f32(v[i].t[k]);
+          s1 += d;
+          s2 = fma(d, d, s2);
+        }
+      }
+    }
+  }
+  const int GV = s.Cg / V;
+  group_sums(s1, s2, s.CV, GV, sl.ng, s.PR, red, grp);
+  const double count = (double)s.HW * s.Cg;
+  if (tid < sl.ng) {
+    const double mean = grp[tid].x / count;
+    double var = grp[tid].y / count - mean * mean;
+    if (var < 0.0) var = 0.0;                            // (NaN stays NaN)
+    const double2 st = make_double2(mean, 1.0 / sqrt(var + eps));
+    grp[tid] = st;
+    stats[(int64_t)b * s.G + sl.g0 + tid] = st;
+  }
+  __syncthreads();
+  if (!on) return;
+  Consts<V> k;
+  load_consts<V>(k, grp - sl.g0, gamma, beta, sl.c0 + cv * V, s.Cg);
+#pragma unroll
+  for (int i = 0; i < NV; i++) {
+    const int p = pr + i * s.PR;
+    if (p < HW) {
+      Vec<T, V> o;
+#pragma unroll
+      for (int j = 0; j < V; j++) o.t[j] = from_f32<T>(act_value<ACT>(fmaf(to_f32(v[i].t[j]) - k.mean[j], k.a[j], k.beta[j])));
+      *(typename Bits<T, V>::type*)(y + base + (int64_t)p * s.C) = o.u;
+    }
+  }
+}
+
+// Backward of a resident slab: dx, and chan[b][2][C] for gn_bwd_finish_kernel.
+template <typename T, int V, int NV, int ACT>
+__global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_bwd_kernel(const T* __restrict__ x, const T* __restrict__ dy,
+                                                                         Shape s, int B, const double2* __restrict__ stats_all,
+                                                                         const float* __restrict__ gamma,
+                                                                         const float* __restrict__ beta, T* __restrict__ dx,
+                                                                         float* __restrict__ chan) {
+  __shared__ float2 red[RES_THREADS * V];
+  __shared__ float2 coef[RES_THREADS];
+  int b, slab;
+  if (!resident_place(s, B, b, slab)) return;
+  const Slab sl = slab_of(s, slab);
+  const double2* stats = stats_all + (int64_t)b * s.G;
+  const int tid = threadIdx.x, cv = tid % s.CV, pr = tid / s.CV, HW = (int)s.HW;
+  const bool on = pr < s.PR && cv * V < sl.nc;
+  const int c = sl.c0 + (on ? cv * V : 0);
+  const int64_t base = (int64_t)b * s.HW * s.C + c;
+  Vec<T, V> vx[NV], vd[NV];
+#pragma unroll
+  for (int i = 0; i < NV; i++) {
+    const int64_t p = min(pr + i * s.PR, HW - 1);
+    vx[i].u = *(const typename Bits<T, V>::type*)(x + base + p * s.C);
+    vd[i].u = *(const typename Bits<T, V>::type*)(dy + base + p * s.C);
+  }
+  Consts<V> k;
+  load_consts<V>(k, stats, gamma, beta, c, s.Cg);
+  const float rstd = (float)stats[c / s.Cg].y;
+  if (on) {
+    float a1[V], a2[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) a1[j] = a2[j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      if (pr + i * s.PR < HW) {
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          const float xf = to_f32(vx[i].t[j]);
+          const float du = du_of<ACT>(xf, to_f32(vd[i].t[j]), k.mean[j], k.a[j], k.beta[j], c + j, s.Cg, stats, gamma);
+          a1[j] += du;
+          a2[j] = fmaf(du, xf - k.mean[j], a2[j]);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < V; j++) red[(pr * s.CV + cv) * V + j] = make_float2(a1[j], a2[j] * rstd);
+  }
+  __syncthreads();
+  const int W = s.CV * V;
+  for (int n = s.PR; n > 1;) {                           // pixel rows: halves onto halves
+    const int h = (n + 1) >> 1;
+    for (int i = tid; i < (n - h) * W; i += RES_THREADS) {
+      if (i % W < sl.nc) {
+        red[i].x += red[i + h * W].x;
+        red[i].y += red[i + h * W].y;
+      }
+    }
+    __syncthreads();
+    n = h;
+  }
+  float* out = chan + (int64_t)b * 2 * s.C;
+  for (int i = tid; i < sl.nc; i += RES_THREADS) {
+    out[sl.c0 + i] = red[i].x;
+    out[s.C + sl.c0 + i] = red[i].y;
+  }
+  if (!dx) return;
+  const float inv = (float)(1.0 / ((double)s.HW * s.Cg));
+  if (s.Cg <= 16) {                                      // a thread per group, else a wave
+    for (int g = tid; g < sl.ng; g += RES_THREADS) {
+      float t1 = 0.f, t2 = 0.f;
+      for (int i = 0; i < s.Cg; i++) {
+        const float w = gamma ? gamma[sl.c0 + g * s.Cg + i] : 1.f;
+        t1 = fmaf(w, red[g * s.Cg + i].x, t1);
+        t2 = fmaf(w, red[g * s.Cg + i].y, t2);
+      }
+      coef[g] = make_float2(t1 * inv, t2 * inv);
+    }
+  } else {
+    for (int g = tid >> 6; g < sl.ng; g += RES_WAVES) {
+      float t1 = 0.f, t2 = 0.f;
+      for (int i = tid & 63; i < s.Cg; i += 64) {
+        const float w = gamma ? gamma[sl.c0 + g * s.Cg + i] : 1.f;
+        t1 = fmaf(w, red[g * s.Cg + i].x, t1);
+        t2 = fmaf(w, red[g * s.Cg + i].y, t2);
+      }
+      t1 = wave_sum(t1);
+      t2 = wave_sum(t2);
+      if ((tid & 63) == 0) coef[g] = make_float2(t1 * inv, t2 * inv);
+    }
+  }
+  __syncthreads();
+  if (!on) return;
+  const float2 m = coef[cv * V / s.Cg];
+  const float q1 = rstd * m.x, q2 = rstd * rstd * m.y;
+#pragma unroll
+  for (int i = 0; i < NV; i++) {
+    const int p = pr + i * s.PR;
+    if (p < HW) {
+      Vec<T, V> o;
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        const float xf = to_f32(vx[i].t[j]);
+        const float du = du_of<ACT>(xf, to_f32(vd[i].t[j]), k.mean[j], k.a[j], k.beta[j], c + j, s.Cg, stats, gamma);
+        o.t[j] = from_f32<T>(fmaf(du, k.a[j], -fmaf(xf - k.mean[j], q2, q1)));
+      }
+      *(typename Bits<T, V>::type*)(dx + base + (int64_t)p * s.C) = o.u;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------
 // Slabs for vectors of V channels; false when they would not start on a vector.
@@ -394,7 +633,7 @@ bool plan_slabs(Shape& s, int V) {
 }
 
 // The widest vector that the channel count, the slabs and the tensors' addresses allow; chunks so that the launch
-// fills the chip eight times over but a thread still walks 16 pixels.
+// fills the chip eight times over but a thread still walks 4 pixels (one round of its loads).
 int plan(Shape& s, int B, int64_t HW, int C, int G, int esize, uintptr_t addr) {
   s.HW = HW;
   s.C = C;
@@ -403,7 +642,7 @@ int plan(Shape& s, int B, int64_t HW, int C, int G, int esize, uintptr_t addr) {
   int V = 16 / esize;
   while (V > 1 && (addr % (V * esize) || !plan_slabs(s, V))) V >>= 1;
   if (V == 1) plan_slabs(s, 1);
-  const int64_t most = (HW + (int64_t)s.PR * 16 - 1) / ((int64_t)s.PR * 16);
+  const int64_t most = (HW + (int64_t)s.PR * 4 - 1) / ((int64_t)s.PR * 4);
   int64_t want = (2048 + (int64_t)B * s.slabs - 1) / ((int64_t)B * s.slabs);
   if (want > most) want = most;
   if (want < 1) want = 1;
@@ -412,24 +651,101 @@ int plan(Shape& s, int B, int64_t HW, int C, int G, int esize, uintptr_t addr) {
   return V;
 }
 
+// Slabs for the resident kernels: whole groups, vectors within a group, at most `most` vectors to a thread.  The widest
+// slab that leaves 512 workgroups (or 256 bytes to a pixel) is taken; narrower ones read less of a memory line at a time
+// but still meet the others of their sample in the XCD's L2.  Below 16 bytes to a pixel that costs more than the launches
+// it saves (16x128x128^2 bf16 in 32 groups, 8 bytes: 74 us against 52), unless a thread holds 8 vectors at most.  Returns
+// the vectors to a thread, 0 where the other kernels are to be used.
+int plan_resident(Shape& s, int& V, int B, int64_t HW, int C, int G, int esize, uintptr_t addr, int most) {
+  s.HW = HW;
+  s.C = C;
+  s.G = G;
+  s.Cg = C / G;
+  s.parts = s.chunks = 1;
+  s.ppc = HW;
+  V = 16 / esize;
+  while (V > 1 && (addr % (V * esize) || s.Cg % V)) V >>= 1;
+  const int GV = s.Cg / V;
+  auto need = [&](int groups) -> int64_t {              // vectors to a thread
+    const int CV = groups * GV;
+    return CV > RES_THREADS ? INT64_MAX : (HW + RES_THREADS / CV - 1) / (RES_THREADS / CV);
+  };
+  if (HW > (1 << 20) || need(1) > most) return 0;
+  int gps = 1;
+  while (gps < G && (int64_t)gps * s.Cg * esize < 256 && need(gps + 1) <= most &&
+         ((int64_t)gps * s.Cg * esize < 16 || (int64_t)B * cdiv(G, gps + 1) >= 512))
+    gps++;
+  if (need(gps) > 8 && gps < G && gps * s.Cg * esize < 16) return 0;
+  s.gps = gps;
+  s.slab_c = gps * s.Cg;
+  s.slabs = cdiv(G, gps);
+  s.CV = gps * GV;
+  s.PR = RES_THREADS / s.CV;
+  return (int)need(gps);
+}
+
 bool shape_ok(int dtype, int B, int64_t HW, int C, int G) {
   return (dtype == MIS_F32 || dtype == MIS_BF16) && B >= 1 && B <= 65535 && HW >= 1 && C >= 1 && G >= 1 && C % G == 0 &&
          C <= 65536 && G <= 65535 && HW <= ((int64_t)1 << 40);
+}
+
+template <typename F> void with_act(int act, F&& f) {
+  switch (act) {
+    case MIS_ACT_RELU: f(std::integral_constant<int, MIS_ACT_RELU>()); break;
+    case MIS_ACT_SILU: f(std::integral_constant<int, MIS_ACT_SILU>()); break;
+    case MIS_ACT_GELU: f(std::integral_constant<int, MIS_ACT_GELU>()); break;
+    default: f(std::integral_constant<int, MIS_ACT_NONE>());
+  }
+}
+
+constexpr int RES_FWD = 32, RES_BWD = 16;               // most vectors to a thread
+
+int resident_grid(const Shape& s, int B) { return (B * s.slabs + 7) / 8 * 8; }
+
+template <typename T, int V>
+void launch_resident_fwd(const T* x, const Shape& s, int nv, int B, const float* gamma, const float* beta, double eps, int act,
+                         T* y, double2* stats, hipStream_t st) {
+  const int grid = resident_grid(s, B);
+  with_act(act, [&](auto a) {
+    constexpr int ACT = decltype(a)::value;
+    if (nv <= 2) gn_resident_kernel<T, V, 2, ACT><<<grid, RES_THREADS, 0, st>>>(x, s, B, eps, gamma, beta, y, stats);
+    else if (nv <= 8) gn_resident_kernel<T, V, 8, ACT><<<grid, RES_THREADS, 0, st>>>(x, s, B, eps, gamma, beta, y, stats);
+    else gn_resident_kernel<T, V, RES_FWD, ACT><<<grid, RES_THREADS, 0, st>>>(x, s, B, eps, gamma, beta, y, stats);
+  });
+}
+
+template <typename T, int V>
+void launch_resident_bwd(const T* x, const T* dy, const Shape& s, int nv, int B, const float* gamma, const float* beta, int act,
+                         const double2* stats, T* dx, float* dgamma, float* dbeta, float* chan, hipStream_t st) {
+  const int grid = resident_grid(s, B);
+  with_act(act, [&](auto a) {
+    constexpr int ACT = decltype(a)::value;
+    if (nv <= 2)
+      gn_resident_bwd_kernel<T, V, 2, ACT><<<grid, RES_THREADS, 0, st>>>(x, dy, s, B, stats, gamma, beta, dx, chan);
+    else if (nv <= 8)
+      gn_resident_bwd_kernel<T, V, 8, ACT><<<grid, RES_THREADS, 0, st>>>(x, dy, s, B, stats, gamma, beta, dx, chan);
+    else
+      gn_resident_bwd_kernel<T, V, RES_BWD, ACT><<<grid, RES_THREADS, 0, st>>>(x, dy, s, B, stats, gamma, beta, dx, chan);
+  });
+  if (dgamma || dbeta)
+    gn_bwd_finish_kernel<<<cdiv(s.C, 64), 256, 0, st>>>(chan, gamma, B, s.C, s.Cg, s.G, 1.0, cdiv(s.C, 64), nullptr, dgamma, dbeta);
 }
 
 template <typename T, int V>
 void launch_fwd(const T* x, const Shape& s, int B, const float* gamma, const float* beta, double eps, int act, T* y,
                 double2* stats, double2* sums, hipStream_t st) {
   const dim3 grid(s.chunks, s.slabs, B);
-  const size_t lds = (size_t)s.PR * s.CV * V * sizeof(double2);
-  gn_sums_kernel<T, V><<<grid, GN_THREADS, lds, st>>>(x, s, sums);
+  auto sum = [&](auto u) {
+    constexpr int U = decltype(u)::value;
+    gn_sums_kernel<T, V, U><<<grid, GN_THREADS, (size_t)s.PR * s.CV * (V / U) * sizeof(double2), st>>>(x, s, sums);
+  };
+  if (s.Cg % V == 0) sum(std::integral_constant<int, V>());
+  else if (V >= 4 && s.Cg % (V / 2) == 0) sum(std::integral_constant<int, (V >= 4 ? V / 2 : 1)>());
+  else sum(std::integral_constant<int, 1>());
   gn_stats_kernel<<<dim3(s.G, B), 64, 0, st>>>(sums, s.chunks * s.parts, s.G, (double)s.HW * s.Cg, eps, stats);
-  switch (act) {
-    case MIS_ACT_RELU: gn_apply_kernel<T, V, MIS_ACT_RELU><<<grid, GN_THREADS, 0, st>>>(x, s, stats, gamma, beta, y); break;
-    case MIS_ACT_SILU: gn_apply_kernel<T, V, MIS_ACT_SILU><<<grid, GN_THREADS, 0, st>>>(x, s, stats, gamma, beta, y); break;
-    case MIS_ACT_GELU: gn_apply_kernel<T, V, MIS_ACT_GELU><<<grid, GN_THREADS, 0, st>>>(x, s, stats, gamma, beta, y); break;
-    default: gn_apply_kernel<T, V, MIS_ACT_NONE><<<grid, GN_THREADS, 0, st>>>(x, s, stats, gamma, beta, y);
-  }
+  with_act(act, [&](auto a) {
+    gn_apply_kernel<T, V, decltype(a)::value><<<grid, GN_THREADS, 0, st>>>(x, s, stats, gamma, beta, y);
+  });
 }
 
 struct BwdBuffers {
@@ -443,21 +759,21 @@ void launch_bwd_act(const T* x, const T* dy, const Shape& s, int B, const float*
   const dim3 grid(s.chunks, s.slabs, B);
   const size_t lds = (size_t)s.PR * s.CV * V * sizeof(float2);
   gn_bwd_sums_kernel<T, V, ACT><<<grid, GN_THREADS, lds, st>>>(x, dy, s, stats, gamma, beta, w.rows);
-  gn_bwd_channels_kernel<<<cdiv(s.C, 32), 256, 0, st>>>(w.rows, B, s.chunks, s.C, w.chan, dgamma, dbeta);
+  gn_bwd_channels_kernel<<<dim3(cdiv(s.C, 32), B), 256, 0, st>>>(w.rows, s.chunks, s.C, w.chan);
+  const int channel_blocks = dgamma || dbeta ? cdiv(s.C, 64) : 0, coef_blocks = dx ? cdiv((int64_t)B * s.G, 4) : 0;
+  if (channel_blocks + coef_blocks > 0)
+    gn_bwd_finish_kernel<<<channel_blocks + coef_blocks, 256, 0, st>>>(w.chan, gamma, B, s.C, s.Cg, s.G, (double)s.HW * s.Cg,
+                                                                      channel_blocks, w.coef, dgamma, dbeta);
   if (!dx) return;
-  gn_bwd_coef_kernel<<<dim3(s.G, B), 64, 0, st>>>(w.chan, gamma, s.C, s.Cg, s.G, (double)s.HW * s.Cg, w.coef);
   gn_bwd_dx_kernel<T, V, ACT><<<grid, GN_THREADS, 0, st>>>(x, dy, s, stats, gamma, beta, w.coef, dx);
 }
 
 template <typename T, int V>
 void launch_bwd(const T* x, const T* dy, const Shape& s, int B, const float* gamma, const float* beta, int act,
                 const double2* stats, T* dx, float* dgamma, float* dbeta, const BwdBuffers& w, hipStream_t st) {
-  switch (act) {
-    case MIS_ACT_RELU: launch_bwd_act<T, V, MIS_ACT_RELU>(x, dy, s, B, gamma, beta, stats, dx, dgamma, dbeta, w, st); break;
-    case MIS_ACT_SILU: launch_bwd_act<T, V, MIS_ACT_SILU>(x, dy, s, B, gamma, beta, stats, dx, dgamma, dbeta, w, st); break;
-    case MIS_ACT_GELU: launch_bwd_act<T, V, MIS_ACT_GELU>(x, dy, s, B, gamma, beta, stats, dx, dgamma, dbeta, w, st); break;
-    default: launch_bwd_act<T, V, MIS_ACT_NONE>(x, dy, s, B, gamma, beta, stats, dx, dgamma, dbeta, w, st);
-  }
+  with_act(act, [&](auto a) {
+    launch_bwd_act<T, V, decltype(a)::value>(x, dy, s, B, gamma, beta, stats, dx, dgamma, dbeta, w, st);
+  });
 }
 
 // Calls f(pointer type tag, vector width) for the planned width.
@@ -516,9 +832,16 @@ int mis_group_norm_act_fwd(const void* x, int dtype, int B, int64_t HW, int C, i
   MIS_REQUIRE((((uintptr_t)x | (uintptr_t)y) & (dtype == MIS_BF16 ? 1 : 3)) == 0 &&
               (((uintptr_t)stats | (uintptr_t)workspace) & 15) == 0, "group_norm_act_fwd: misaligned pointer");
   Shape s;
-  const int V = plan(s, B, HW, C, G, dtype == MIS_BF16 ? 2 : 4, (uintptr_t)x | (uintptr_t)y | 16);
+  const int es = dtype == MIS_BF16 ? 2 : 4;
+  const uintptr_t addr = (uintptr_t)x | (uintptr_t)y | 16;
+  int V;
+  const int nv = plan_resident(s, V, B, HW, C, G, es, addr, RES_FWD);
+  if (!nv) V = plan(s, B, HW, C, G, es, addr);
   with_vector(dtype, V, [&](auto* t, auto v) {
     typedef std::remove_pointer_t<decltype(t)> T;
+    if (nv)
+      return launch_resident_fwd<T, decltype(v)::value>((const T*)x, s, nv, B, gamma, beta, eps, act, (T*)y, (double2*)stats,
+                                                        (hipStream_t)stream);
     launch_fwd<T, decltype(v)::value>((const T*)x, s, B, gamma, beta, eps, act, (T*)y, (double2*)stats, (double2*)workspace,
                                       (hipStream_t)stream);
   });
@@ -542,7 +865,11 @@ int mis_group_norm_act_bwd(const void* x, const void* dy, int dtype, int B, int6
   MIS_REQUIRE((((uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx) & (dtype == MIS_BF16 ? 1 : 3)) == 0 &&
               (((uintptr_t)stats | (uintptr_t)workspace) & 15) == 0, "group_norm_act_bwd: misaligned pointer");
   Shape s;
-  const int V = plan(s, B, HW, C, G, dtype == MIS_BF16 ? 2 : 4, (uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx | 16);
+  const int es = dtype == MIS_BF16 ? 2 : 4;
+  const uintptr_t addr = (uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx | 16;
+  int V;
+  const int nv = plan_resident(s, V, B, HW, C, G, es, addr, RES_BWD);
+  if (!nv) V = plan(s, B, HW, C, G, es, addr);
   BwdBuffers w;
   char* ws = (char*)workspace;
   w.rows = (float*)ws;
@@ -552,6 +879,10 @@ int mis_group_norm_act_bwd(const void* x, const void* dy, int dtype, int B, int6
   w.coef = (float2*)ws;
   with_vector(dtype, V, [&](auto* t, auto v) {
     typedef std::remove_pointer_t<decltype(t)> T;
+    if (nv)
+      return launch_resident_bwd<T, decltype(v)::value>((const T*)x, (const T*)dy, s, nv, B, gamma, beta, act,
+                                                        (const double2*)stats, (T*)dx, dgamma, dbeta, w.chan,
+                                                        (hipStream_t)stream);
     launch_bwd<T, decltype(v)::value>((const T*)x, (const T*)dy, s, B, gamma, beta, act, (const double2*)stats, (T*)dx,
                                       dgamma, dbeta, w, (hipStream_t)stream);
   });

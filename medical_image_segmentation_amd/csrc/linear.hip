@@ -59,8 +59,9 @@ template <> struct Mma<float> {
 // Tiles staged straight from memory into LDS (16-byte chunks; sizes, strides and addresses multiples of 16 bytes).
 //
 // A workgroup of WP x WQ waves owns TP x TQ outputs and walks r in steps of 128 bytes (64 bf16, 32 float32).  Two
-// stages of LDS: while the matrix instructions work on one, buffer loads with an LDS destination fill the other; one
-// barrier a stage.  Chunks outside the operand get an offset behind the buffer's end and arrive as zeros.
+// stages of LDS (four for the 64-edge, which is used where few workgroups are left to hide a load behind): while the
+// matrix instructions work on one, buffer loads with an LDS destination fill the others; one barrier a stage.  Chunks
+// outside the operand get an offset behind the buffer's end and arrive as zeros.
 //
 // Rows of an operand that is contiguous in r are 128 bytes of LDS; a fragment read takes the same 16-byte chunk of 16
 // rows, so chunk c of row i lies at c ^ ((i / 2) % 8): 16 rows, 16 different 16-byte windows of the 256 bytes of banks.
@@ -200,7 +201,14 @@ struct Grid {
   __host__ __device__ int launch() const { return (total() + XCDS - 1) / XCDS * XCDS; }
 };
 
-template <typename T, int TP, int TQ, int WP, int WQ, bool PTR, bool QTR, int MODE>
+// All but the last N loads of this wave have arrived, its LDS reads are done, and all waves are here.
+template <int N> __device__ __forceinline__ void wait_and_meet() {
+#ifdef __HIP_DEVICE_COMPILE__
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+#endif
+}
+
+template <typename T, int TP, int TQ, int WP, int WQ, int STAGES, bool PTR, bool QTR, int MODE>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void lin_tile_kernel(Operand<T> P, Operand<T> Q, int64_t R, Grid grid,
                                                                    Epilogue<T> e) {
   constexpr int THREADS = 64 * WP * WQ, BP = TP / WP / 16, BQ = TQ / WQ / 16, K = ROW_BYTES / (int)sizeof(T);
@@ -228,20 +236,20 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void lin_tile_kernel(Operand<T> P,
   const T* qp = Q.p + (int64_t)q0 * Q.s_row + r0 * Q.s_k;
 
   f32x4 acc[BP][BQ] = {};
-  if (r0 < r1) {                             // (every load is waited for inside the loop)
-    sp.issue(pp, r1 - r0, lds);
-    sq.issue(qp, r1 - r0, lds + TP * ROW_BYTES);
-  }
+  int64_t left = r1 - r0;                   // from the next stage to be loaded on; stages behind the end are loaded as zeros
+  auto load = [&](int buf) {
+    sp.issue(pp, left, lds + buf * STAGE);
+    sq.issue(qp, left, lds + buf * STAGE + TP * ROW_BYTES);
+    pp += K * P.s_k;
+    qp += K * Q.s_k;
+    left -= K;
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; i++) load(i);
   int cur = 0;
-  for (int64_t r = r0; r < r1; r += K, cur ^= 1) {
-    __syncthreads();                        // this stage has arrived; nobody reads the other one any more
-    if (r + K < r1) {
-      char* next = lds + (cur ^ 1) * STAGE;
-      pp += K * P.s_k;
-      qp += K * Q.s_k;
-      sp.issue(pp, r1 - r - K, next);
-      sq.issue(qp, r1 - r - K, next + TP * ROW_BYTES);
-    }
+  for (int64_t r = r0; r < r1; r += K) {
+    wait_and_meet<(STAGES - 2) * (sp.N + sq.N)>();       // this stage is here; nobody reads the one before it any more
+    load(cur == 0 ? STAGES - 1 : cur - 1);
     const char* tp = lds + cur * STAGE;
     const char* tq = tp + TP * ROW_BYTES;
 #pragma unroll
@@ -256,7 +264,9 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void lin_tile_kernel(Operand<T> P,
 #pragma unroll
         for (int j = 0; j < BQ; j++) acc[i][j] = multiply(a[i], b[j], acc[i][j], T());
     }
+    cur = cur + 1 == STAGES ? 0 : cur + 1;
   }
+  wait_and_meet<0>();                       // (no load may reach LDS that this workgroup no longer owns)
 
   // A lane has p = 4 g + 0..3 of every 16 x 16 block, q = lane % 16.  For 16-byte accesses in bf16 the lanes of two
   // neighbouring blocks trade halves (v_permlane16_swap): 8 consecutive p of one block each.
@@ -314,7 +324,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void lin_tile_kernel(Operand<T> P,
         }
       }
       if constexpr (MODE == DZ) {
-        float* colsum = (float*)(lds + 2 * STAGE);           // [WQ][TP]
+          float* colsum = (float*)lds;                        // [WQ][TP], the stages are done
 #pragma unroll
         for (int k = 0; k < NV; k++) {
           const float s = row16_sum(cs[k]);
@@ -324,7 +334,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void lin_tile_kernel(Operand<T> P,
     }
   });
   if constexpr (MODE == DZ) {
-    const float* colsum = (const float*)(lds + 2 * STAGE);
+    const float* colsum = (const float*)lds;
     __syncthreads();
     for (int c = threadIdx.x; c < TP && p0 + c < P.rows; c += THREADS) {
       float s = 0.f;
@@ -434,13 +444,70 @@ __global__ __launch_bounds__(256) void lin_any_kernel(Operand<T> P, Operand<T> Q
   }
 }
 
-// out[i] = sum over the splits, in their order
-template <typename T>
-__global__ __launch_bounds__(256) void lin_join_kernel(const float* __restrict__ part, int splits, int64_t n, T* __restrict__ out) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    float s = 0.f;
-    for (int k = 0; k < splits; k++) s += part[k * n + i];
-    out[i] = from_f32<T>(s);
+// The epilogue for a product whose sum was split: part [splits][Q][P] added up in a fixed order.  Block = 64 consecutive
+// p x LANES, rows_per_block q rows one after another: few splits: a lane to a q row; many (LANES = 16): the lanes share
+// the splits of one q row.  DZ leaves rows[block of JOIN_Q q][p].
+constexpr int JOIN_Q = 16, JOIN_FEW = 8;
+template <typename T, int MODE, bool FEW>
+__global__ __launch_bounds__(FEW ? 256 : 1024) void lin_join_kernel(const float* __restrict__ part, int splits, int P, int Q,
+                                                                    int rows_per_block, Epilogue<T> e) {
+  constexpr int LANES = FEW ? 4 : 16;
+  __shared__ float red[LANES][64];
+  const int p_blocks = (P + 63) / 64, q_block = blockIdx.x / p_blocks, c = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int p = (blockIdx.x - q_block * p_blocks) * 64 + c;
+  const int64_t n = (int64_t)P * Q;
+  const int qa = q_block * rows_per_block, qb = min(qa + rows_per_block, Q);
+  const bool in = p < P;
+  const float bias = (MODE == FWD || MODE == DZ) && e.bias && in ? e.bias[p] : 0.f;
+  float cs = 0.f;
+  with_act(MODE == FWD || MODE == DZ ? e.act : MIS_ACT_NONE, [&](auto act) {
+    constexpr int ACT = decltype(act)::value;
+    auto finish = [&](int q, float v) {
+      if constexpr (MODE == FWD) {
+        v = act_value<ACT>(v + bias);
+        if (e.other) v += to_f32(e.other[q * e.ld + p]);
+      }
+      if constexpr (MODE == DZ) {
+        v = to_f32(e.other[q * e.ld + p]) * act_slope<ACT>(v + bias);
+        cs += v;
+      }
+      e.out[(int64_t)q * P + p] = from_f32<T>(v);
+    };
+    if constexpr (FEW) {
+      if (in)
+        for (int q = qa + w; q < qb; q += LANES) {
+          float v = 0.f;
+#pragma unroll
+          for (int k = 0; k < JOIN_FEW; k++)
+            if (k < splits) v += part[k * n + (int64_t)q * P + p];
+          finish(q, v);
+        }
+    } else {
+      for (int q = qa; q < qb; q++) {
+        float v = 0.f;
+        if (in) {
+#pragma unroll 8
+          for (int k = w; k < splits; k += LANES) v += part[k * n + (int64_t)q * P + p];
+        }
+        red[w][c] = v;
+        __syncthreads();
+        if (w == 0 && in) {
+#pragma unroll
+          for (int k = 1; k < LANES; k++) v += red[k][c];
+          finish(q, v);
+        }
+        __syncthreads();
+      }
+    }
+  });
+  if constexpr (MODE == DZ) {
+    red[w][c] = cs;
+    __syncthreads();
+    if (w == 0 && in) {
+#pragma unroll
+      for (int k = 1; k < LANES; k++) cs += red[k][c];
+      e.rows[(int64_t)q_block * P + p] = cs;
+    }
   }
 }
 
@@ -463,9 +530,51 @@ __global__ __launch_bounds__(256) void lin_colsum_kernel(const T* __restrict__ d
 // ---------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------
-// Output tile of a product: the q rows that one row of partial sums covers is the kernel's TQ.
 enum Tile { ANY64, T64, T128, T256 };
 int tile_edge(Tile t) { return t == T256 ? 256 : t == T128 ? 128 : 64; }
+
+// How a product is cut up: the edge of the output tiles, and parts of the sum (joined by a second launch).
+struct Cut {
+  Tile tile;
+  int splits;
+  int64_t per;          // r per split, a multiple of a stage
+  int row_tiles() const { return splits > 1 ? JOIN_Q : tile_edge(tile); }      // q rows behind a row of partial sums
+};
+
+// The cheapest by a model of the time in microseconds: rounds of workgroups over the chip's 256 CUs; a round = start,
+// epilogue and its stages, a stage at the matrix rate of the tile (shared by the workgroups of a CU) or, for a lone
+// workgroup, at the time a load takes; for a split sum the second launch, and the parts written and read.  The constants
+// are fitted to 78 products of 1 to 10^6 rows and 24 to 4096 columns, forward and both backward ones, bf16 and float32,
+// each measured in all cuts: the choice is 2 % slower than the best cut on average, 30 % at worst (a 20 us product).
+Cut pick_cut(int esize, bool staged, int64_t p, int64_t q, int64_t r) {
+  struct Rate { double full, alone; int at_a_time; };
+  static const Rate rates[] = {{1.5, 1.5, 3}, {0.185, 0.46, 3}, {0.50, 0.90, 2}, {2.0, 0.90, 1}};      // by Tile
+  const int K = ROW_BYTES / esize;
+  const int64_t stages = (r + K - 1) / K;
+  Cut best{ANY64, 1, stages * K};
+  double least = 1e300;
+  for (int t = staged ? T64 : ANY64; t <= (staged ? T256 : ANY64); t++) {
+    const int edge = tile_edge((Tile)t), slots = 256 * rates[t].at_a_time;
+    const int64_t tiles = (int64_t)cdiv(p, edge) * cdiv(q, edge);
+    auto round_us = [&](int64_t wgs, int64_t per) {
+      const double share = wgs > 256 ? wgs / 256.0 : 1.0, full = rates[t].full * (esize == 4 ? 2.8 : 1.0) * share;
+      return 2.9 + 3e-5 * edge * edge * share + per * (full > rates[t].alone ? full : rates[t].alone);
+    };
+    for (int s = 1; s <= 1024; s *= 2) {
+      const int64_t per = (stages + s - 1) / s;
+      const int splits = (int)((stages + per - 1) / per);
+      if (s > 1 && (splits == 1 || per < 2 || tiles * splits > 4096)) break;
+      const int64_t wgs = tiles * splits, rounds = (wgs + slots - 1) / slots;
+      double us = (rounds - 1) * round_us(slots, per) + round_us(wgs - (rounds - 1) * slots, per);
+      if (splits > 1) us += 2.9 + 3.1e-6 * splits * p * q;
+      if (us < least) {
+        least = us;
+        best = Cut{(Tile)t, splits, per * K};
+      }
+    }
+  }
+  return best;
+}
 
 // Whether the staged kernels take these: everything in 16-byte chunks.
 template <typename T> bool chunked(const Operand<T>& o, int64_t R) {
@@ -475,68 +584,79 @@ template <typename T> bool chunked(const Operand<T>& o, int64_t R) {
   return o.rows % V == 0 && o.s_k % V == 0 && o.s_k * (int64_t)sizeof(T) * 64 < 0x7FFFFF00;
 }
 
-Tile pick_tile(int64_t p, int64_t q, int splits) {
-  if ((int64_t)cdiv(p, 256) * cdiv(q, 256) * splits >= 256) return T256;
-  if ((int64_t)cdiv(p, 128) * cdiv(q, 128) * splits >= 256) return T128;
-  return T64;
+template <typename T> bool staged(const Operand<T>& P, const Operand<T>& Q, int64_t R, const Epilogue<T>& e) {
+  constexpr int V = 16 / sizeof(T);
+  return chunked(P, R) && chunked(Q, R) && P.rows % V == 0 && (((uintptr_t)e.other | (uintptr_t)e.out) & 15) == 0 &&
+         (!e.other || e.ld % V == 0);
 }
 
-template <typename T, int TP, int TQ, int WP, int WQ, bool PTR, bool QTR, int MODE>
-int launch_tile(const Operand<T>& P, const Operand<T>& Q, int64_t R, int splits, int64_t per, const Epilogue<T>& e, hipStream_t st) {
-  constexpr int LDS = 2 * (TP + TQ) * ROW_BYTES + (MODE == DZ ? WQ * TP * 4 : 0);
+template <typename T, int TP, int TQ, int WP, int WQ, int STAGES, bool PTR, bool QTR, int MODE>
+int launch_tile(const Operand<T>& P, const Operand<T>& Q, int64_t R, const Cut& cut, const Epilogue<T>& e, hipStream_t st) {
+  constexpr int LDS = STAGES * (TP + TQ) * ROW_BYTES;
   if constexpr (LDS > 65536) {
     static thread_local bool raised[64] = {};
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev >= 64) return 1;
     if (!raised[dev]) {
-      if (hipFuncSetAttribute((const void*)lin_tile_kernel<T, TP, TQ, WP, WQ, PTR, QTR, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return 1;
+      if (hipFuncSetAttribute((const void*)lin_tile_kernel<T, TP, TQ, WP, WQ, STAGES, PTR, QTR, MODE>,
+                              hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
+        return 1;
       raised[dev] = true;
     }
   }
-  const Grid g{cdiv(P.rows, TP), cdiv(Q.rows, TQ), splits, per};
-  lin_tile_kernel<T, TP, TQ, WP, WQ, PTR, QTR, MODE><<<g.launch(), 64 * WP * WQ, LDS, st>>>(P, Q, R, g, e);
+  const Grid g{cdiv(P.rows, TP), cdiv(Q.rows, TQ), cut.splits, cut.per};
+  lin_tile_kernel<T, TP, TQ, WP, WQ, STAGES, PTR, QTR, MODE><<<g.launch(), 64 * WP * WQ, LDS, st>>>(P, Q, R, g, e);
   return 0;
 }
 
 template <typename T, bool PTR, bool QTR, int MODE>
-int launch_staged(Tile tile, const Operand<T>& P, const Operand<T>& Q, int64_t R, int splits, int64_t per, const Epilogue<T>& e,
-                  hipStream_t st) {
-  switch (tile) {
-    case T256: return launch_tile<T, 256, 256, 2, 4, PTR, QTR, MODE>(P, Q, R, splits, per, e, st);
-    case T128: return launch_tile<T, 128, 128, 2, 2, PTR, QTR, MODE>(P, Q, R, splits, per, e, st);
-    default: return launch_tile<T, 64, 64, 2, 2, PTR, QTR, MODE>(P, Q, R, splits, per, e, st);
+int launch_cut(const Operand<T>& P, const Operand<T>& Q, int64_t R, const Cut& cut, const Epilogue<T>& e, hipStream_t st) {
+  switch (cut.tile) {
+    case T256: return launch_tile<T, 256, 256, 2, 4, 2, PTR, QTR, MODE>(P, Q, R, cut, e, st);
+    case T128: return launch_tile<T, 128, 128, 2, 2, 2, PTR, QTR, MODE>(P, Q, R, cut, e, st);
+    case T64: return launch_tile<T, 64, 64, 2, 2, 4, PTR, QTR, MODE>(P, Q, R, cut, e, st);
+    default:
+      lin_any_kernel<T, MODE><<<dim3(cdiv(P.rows, ANY_T) * cdiv(Q.rows, ANY_T), cut.splits), 256, 0, st>>>(P, Q, R, cut.per, e);
+      return 0;
   }
 }
 
+// out = epilogue(P Q^T); `e.rows` takes DZ's partial sums, `part` the parts of a split sum.
 template <typename T, bool PTR, bool QTR, int MODE>
-int launch_product(Tile tile, const Operand<T>& P, const Operand<T>& Q, int64_t R, int splits, const Epilogue<T>& e, hipStream_t st) {
-  const int64_t per = ((R + splits - 1) / splits + 63) / 64 * 64;
-  if (tile != ANY64) return launch_staged<T, PTR, QTR, MODE>(tile, P, Q, R, splits, per, e, st);
-  lin_any_kernel<T, MODE><<<dim3(cdiv(P.rows, ANY_T) * cdiv(Q.rows, ANY_T), splits), 256, 0, st>>>(P, Q, R, per, e);
+int product(const Operand<T>& P, const Operand<T>& Q, int64_t R, const Cut& cut, Epilogue<T> e, float* part, hipStream_t st) {
+  if (cut.splits == 1) return launch_cut<T, PTR, QTR, MODE>(P, Q, R, cut, e, st);
+  const Epilogue<T> partial{nullptr, nullptr, 0, nullptr, part, MIS_ACT_NONE};
+  if (launch_cut<T, PTR, QTR, PARTIAL>(P, Q, R, cut, partial, st)) return 1;
+  const int rpb = MODE == DZ ? JOIN_Q : cut.splits <= JOIN_FEW ? 4 : 1, grid = cdiv(P.rows, 64) * cdiv(Q.rows, rpb);
+  if (cut.splits <= JOIN_FEW) lin_join_kernel<T, MODE, true><<<grid, 256, 0, st>>>(part, cut.splits, P.rows, Q.rows, rpb, e);
+  else lin_join_kernel<T, MODE, false><<<grid, 1024, 0, st>>>(part, cut.splits, P.rows, Q.rows, rpb, e);
   return 0;
 }
 
-// Parts of the long sum of dW: enough workgroups to fill the chip twice, at least 256 rows to a part.
-int wgrad_splits(int64_t M, int64_t N, int64_t K) {
-  const int64_t tiles = (int64_t)cdiv(N, ANY_T) * cdiv(K, ANY_T);
-  int64_t s = (512 + tiles - 1) / tiles;
-  const int64_t most = (M + 255) / 256;
-  if (s > most) s = most;
-  return (int)(s < 1 ? 1 : s);
+// Sizes of a call's scratch.  Whether a product can be staged depends on addresses and strides that the size query does
+// not know: the larger of both ways counts.
+size_t part_bytes(int esize, int64_t p, int64_t q, int64_t r) {
+  size_t most = 0;
+  for (int staged = 0; staged < 2; staged++) {
+    const Cut c = pick_cut(esize, staged, p, q, r);
+    const size_t n = c.splits > 1 ? (size_t)c.splits * p * q * sizeof(float) : 0;
+    if (n > most) most = n;
+  }
+  return align256(most);
 }
 
 struct BwdPlan {
   size_t dz, rows, part, total;
-  int splits;
 };
 
 BwdPlan bwd_plan(int dtype, int64_t M, int64_t N, int64_t K, int act) {
   BwdPlan p;
-  const size_t es = dtype == MIS_BF16 ? 2 : 4;
-  p.splits = wgrad_splits(M, N, K);
+  const int es = dtype == MIS_BF16 ? 2 : 4;
   p.dz = act == MIS_ACT_NONE ? 0 : align256((size_t)M * N * es);
-  p.rows = align256((size_t)(act == MIS_ACT_NONE ? cdiv(M, SUM_ROWS) : cdiv(M, ANY_T)) * N * sizeof(float));
-  p.part = p.splits > 1 ? align256((size_t)p.splits * N * K * sizeof(float)) : 0;
+  p.rows = align256((size_t)(act == MIS_ACT_NONE ? cdiv(M, SUM_ROWS) : cdiv(M, pick_cut(es, false, N, M, K).splits > 1 || pick_cut(es, true, N, M, K).splits > 1 ? JOIN_Q : 64)) * N * sizeof(float));
+  p.part = part_bytes(es, K, M, N);
+  for (size_t n : {part_bytes(es, K, N, M), act == MIS_ACT_NONE ? (size_t)0 : part_bytes(es, N, M, K)})
+    if (n > p.part) p.part = n;
   p.total = p.dz + p.rows + p.part;
   return p;
 }
@@ -553,19 +673,11 @@ bool aligned(int dtype, std::initializer_list<const void*> ps) {
 }
 
 template <typename T>
-Tile tile_for(const Operand<T>& P, const Operand<T>& Q, int64_t R, const Epilogue<T>& e, int splits) {
-  constexpr int V = 16 / sizeof(T);
-  const bool ok = chunked(P, R) && chunked(Q, R) && P.rows % V == 0 && (((uintptr_t)e.other | (uintptr_t)e.out) & 15) == 0 &&
-                  (!e.other || e.ld % V == 0);
-  return ok ? pick_tile(P.rows, Q.rows, splits) : ANY64;
-}
-
-template <typename T>
 int forward(const T* x, int64_t ldx, const T* w, const float* bias, const T* r, int64_t ldr, int64_t M, int64_t N, int64_t K,
-            int act, T* y, hipStream_t st) {
+            int act, T* y, char* ws, hipStream_t st) {
   const Operand<T> P{w, K, 1, (int)N}, Q{x, ldx, 1, (int)M};
   const Epilogue<T> e{bias, r, ldr, y, nullptr, act};
-  return launch_product<T, false, false, FWD>(tile_for(P, Q, K, e, 1), P, Q, K, 1, e, st);
+  return product<T, false, false, FWD>(P, Q, K, pick_cut(sizeof(T), staged(P, Q, K, e), N, M, K), e, (float*)ws, st);
 }
 
 template <typename T>
@@ -580,27 +692,24 @@ int backward(const T* x, int64_t ldx, const T* w, const float* bias, const T* dy
   if (act != MIS_ACT_NONE) {
     const Operand<T> P{w, K, 1, (int)N}, Q{x, ldx, 1, (int)M};
     const Epilogue<T> e{bias, dy, ldd, dz, rows, act};
-    const Tile tile = tile_for(P, Q, K, e, 1);
-    if (launch_product<T, false, false, DZ>(tile, P, Q, K, 1, e, st)) return 1;
+    const Cut cut = pick_cut(sizeof(T), staged(P, Q, K, e), N, M, K);
+    if (product<T, false, false, DZ>(P, Q, K, cut, e, part, st)) return 1;
     z = dz;
     ldz = N;
-    if (db) launch_reduce_partials(rows, cdiv(M, tile_edge(tile)), (int)N, db, st);
+    if (db) launch_reduce_partials(rows, cdiv(M, cut.row_tiles()), (int)N, db, st);
   } else if (db) {
     lin_colsum_kernel<T><<<dim3(cdiv(M, SUM_ROWS), cdiv(N, 64)), 256, 0, st>>>(dy, ldd, M, (int)N, rows);
     launch_reduce_partials(rows, cdiv(M, SUM_ROWS), (int)N, db, st);
   }
   if (dx) {
     const Operand<T> P{w, 1, K, (int)K}, Q{z, ldz, 1, (int)M};
-    const Epilogue<T> e{nullptr, nullptr, 0, dx, nullptr, 0};
-    if (launch_product<T, true, false, STORE>(tile_for(P, Q, N, e, 1), P, Q, N, 1, e, st)) return 1;
+    const Epilogue<T> e{nullptr, nullptr, 0, dx, nullptr, MIS_ACT_NONE};
+    if (product<T, true, false, STORE>(P, Q, N, pick_cut(sizeof(T), staged(P, Q, N, e), K, M, N), e, part, st)) return 1;
   }
   if (dw) {
     const Operand<T> P{x, 1, ldx, (int)K}, Q{z, 1, ldz, (int)N};
-    const Epilogue<T> e{nullptr, nullptr, 0, dw, part, 0};
-    const Tile tile = tile_for(P, Q, M, e, p.splits);
-    if (p.splits == 1) return launch_product<T, true, true, STORE>(tile, P, Q, M, 1, e, st);
-    if (launch_product<T, true, true, PARTIAL>(tile, P, Q, M, p.splits, e, st)) return 1;
-    lin_join_kernel<T><<<ew_grid(N * K, 256), 256, 0, st>>>(part, p.splits, N * K, dw);
+    const Epilogue<T> e{nullptr, nullptr, 0, dw, nullptr, MIS_ACT_NONE};
+    if (product<T, true, true, STORE>(P, Q, M, pick_cut(sizeof(T), staged(P, Q, M, e), K, N, M), e, part, st)) return 1;
   }
   return 0;
 }
@@ -609,20 +718,28 @@ int backward(const T* x, int64_t ldx, const T* w, const float* bias, const T* dy
 
 extern "C" {
 
+size_t mis_linear_act_fwd_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
+  if (!sizes_ok(dtype, M, N, K)) return 0;
+  const size_t n = part_bytes(dtype == MIS_BF16 ? 2 : 4, N, M, K);
+  return n ? n : 256;
+}
+
 int mis_linear_act_fwd(const void* x, int64_t ldx, const void* w, const float* bias, const void* residual, int64_t ldr, int dtype,
-                       int64_t M, int64_t N, int64_t K, int act, void* y, mis_stream_t stream) {
-  MIS_REQUIRE(x && w && y, "linear_act_fwd: null pointer");
+                       int64_t M, int64_t N, int64_t K, int act, void* y, void* workspace, mis_stream_t stream) {
+  MIS_REQUIRE(x && w && y && workspace, "linear_act_fwd: null pointer");
   MIS_REQUIRE(sizes_ok(dtype, M, N, K), "linear_act_fwd: bad dtype or sizes (M=%lld N=%lld K=%lld)", (long long)M, (long long)N,
               (long long)K);
   MIS_REQUIRE(ldx >= K && (!residual || ldr >= N), "linear_act_fwd: row stride below the row length");
   MIS_REQUIRE(act >= MIS_ACT_NONE && act <= MIS_ACT_GELU, "linear_act_fwd: unknown activation %d", act);
-  MIS_REQUIRE(aligned(dtype, {x, w, residual, y}), "linear_act_fwd: misaligned pointer");
+  MIS_REQUIRE(aligned(dtype, {x, w, residual, y}) && ((uintptr_t)workspace & 15) == 0, "linear_act_fwd: misaligned pointer");
   hipStream_t st = (hipStream_t)stream;
   int rc;
   if (dtype == MIS_BF16)
-    rc = forward((const bf16*)x, ldx, (const bf16*)w, bias, (const bf16*)residual, ldr, M, N, K, act, (bf16*)y, st);
+    rc = forward((const bf16*)x, ldx, (const bf16*)w, bias, (const bf16*)residual, ldr, M, N, K, act, (bf16*)y,
+                 (char*)workspace, st);
   else
-    rc = forward((const float*)x, ldx, (const float*)w, bias, (const float*)residual, ldr, M, N, K, act, (float*)y, st);
+    rc = forward((const float*)x, ldx, (const float*)w, bias, (const float*)residual, ldr, M, N, K, act, (float*)y,
+                 (char*)workspace, st);
   MIS_REQUIRE(rc == 0, "linear_act_fwd: the device refuses the kernel's shared memory");
   MIS_CHECK_LAUNCH("linear_act_fwd");
   return MIS_OK;

@@ -1953,8 +1953,9 @@ class LinearActFn(torch.autograd.Function):
         if M:
             nbytes = (M * K + N * K + M * N * (1 if r2 is None else 2)) * x.element_size()
             with _on_device_of(x), _prof("linear_act_fwd", 2 * M * N * K, nbytes):
+                ws = _scratch(query("mis_linear_act_fwd_workspace_bytes", _dt(x), M, N, K), x.device)
                 call("mis_linear_act_fwd", x2.data_ptr(), ldx, w.data_ptr(), _p(bias), _p(r2), ldr, _dt(x), M, N, K, act,
-                     y.data_ptr(), _stream())
+                     y.data_ptr(), ws.data_ptr(), _stream())
         ctx.save_for_backward(x, w, bias)
         ctx.act = act
         return y

@@ -28,10 +28,10 @@ def test_group_norm_c_entry():
 
 
 def test_linear_c_entry():
-    fwd = lambda *, x=P, ldx=8, w=P, r=None, ldr=0, dtype=0, M=4, N=8, K=8, act=0, y=P: (  # noqa: E731
-        x, ldx, w, None, r, ldr, dtype, M, N, K, act, y, None)
+    fwd = lambda *, x=P, ldx=8, w=P, r=None, ldr=0, dtype=0, M=4, N=8, K=8, act=0, y=P, ws=P: (  # noqa: E731
+        x, ldx, w, None, r, ldr, dtype, M, N, K, act, y, ws, None)
     for bad in (dict(x=None), dict(w=None), dict(y=None), dict(ldx=7), dict(r=P, ldr=7), dict(dtype=3), dict(M=0), dict(N=0),
-                dict(K=0), dict(M=1 << 31), dict(act=5), dict(x=ctypes.c_void_p(4098)), dict(K=1 << 21, ldx=1 << 21)):
+                dict(K=0), dict(M=1 << 31), dict(act=5), dict(x=ctypes.c_void_p(4098)), dict(K=1 << 21, ldx=1 << 21), dict(ws=None)):
         _refused("mis_linear_act_fwd", *fwd(**bad), match="linear_act_fwd")
     bwd = lambda *, x=P, ldx=8, dy=P, ldd=8, M=4, ws=P, act=0: (  # noqa: E731
         x, ldx, P, None, dy, ldd, 1, M, 8, 8, act, None, None, None, ws, None)
