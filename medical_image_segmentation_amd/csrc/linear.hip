@@ -25,7 +25,9 @@ template <typename T> struct Epilogue {
   const float* bias;        // [p]
   const T* other;           // residual (FWD, may be null) or dy (DZ): [q][p], row stride ld
   int64_t ld;
-  T* out;                   // [q][p] dense
+  T* out;                   // [q][p], row stride ld_out; columns from the operand's rows up to `cols` are set to zero
+  int64_t ld_out;
+  int cols;
   float* rows;              // DZ: sums over a tile's q, [q tile][p];  PARTIAL: [split][q][p]
   int act;
 };
@@ -208,7 +210,7 @@ template <int N> __device__ __forceinline__ void wait_and_meet() {
 #endif
 }
 
-template <typename T, int TP, int TQ, int WP, int WQ, int STAGES, bool PTR, bool QTR, int MODE>
+template <typename T, int TP, int TQ, int WP, int WQ, int STAGES, bool PTR, bool QTR, int MODE, bool WIDE>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void lin_tile_kernel(Operand<T> P, Operand<T> Q, int64_t R, Grid grid,
                                                                    Epilogue<T> e) {
   constexpr int THREADS = 64 * WP * WQ, BP = TP / WP / 16, BQ = TQ / WQ / 16, K = ROW_BYTES / (int)sizeof(T);
@@ -270,14 +272,15 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void lin_tile_kernel(Operand<T> P,
 
   // A lane has p = 4 g + 0..3 of every 16 x 16 block, q = lane % 16.  For 16-byte accesses in bf16 the lanes of two
   // neighbouring blocks trade halves (v_permlane16_swap): 8 consecutive p of one block each.
-  constexpr bool WIDE = sizeof(T) == 2 && MODE != PARTIAL;
-  constexpr int NV = WIDE ? 8 : 4, PAIRS = WIDE ? BP / 2 : BP;
+  // WIDE false: some row or column does not fit 16-byte accesses; the same values, element by element.
+  constexpr bool TRADE = sizeof(T) == 2 && MODE != PARTIAL;
+  constexpr int NV = TRADE ? 8 : 4, PAIRS = TRADE ? BP / 2 : BP;
+  const int cols = MODE == PARTIAL ? P.rows : e.cols;
   with_act(MODE == FWD || MODE == DZ ? e.act : MIS_ACT_NONE, [&](auto act) {
     constexpr int ACT = decltype(act)::value;
 #pragma unroll
     for (int i = 0; i < PAIRS; i++) {
-      const int pl = wp + (WIDE ? 32 * i + 16 * (g & 1) + 8 * (g >> 1) : 16 * i + 4 * g), p = p0 + pl;
-      const bool in_p = p < P.rows;
+      const int pl = wp + (TRADE ? 32 * i + 16 * (g & 1) + 8 * (g >> 1) : 16 * i + 4 * g), p = p0 + pl;
       float bias[NV], cs[NV];
 #pragma unroll
       for (int k = 0; k < NV; k++) {
@@ -285,13 +288,13 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void lin_tile_kernel(Operand<T> P,
         cs[k] = 0.f;
       }
       if constexpr (MODE == FWD || MODE == DZ)
-        if (e.bias && in_p)
+        if (e.bias && p < P.rows)
 #pragma unroll
-          for (int k = 0; k < NV; k++) bias[k] = e.bias[p + k];
+          for (int k = 0; k < NV; k++) bias[k] = WIDE || p + k < P.rows ? e.bias[p + k] : 0.f;
 #pragma unroll
       for (int j = 0; j < BQ; j++) {
         float v[NV];
-        if constexpr (WIDE) {
+        if constexpr (TRADE) {
 #pragma unroll
           for (int k = 0; k < 4; k++) {
             const auto s = __builtin_amdgcn_permlane16_swap(as_bits(acc[2 * i][j][k]), as_bits(acc[2 * i + 1][j][k]), false, false);
@@ -303,28 +306,48 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void lin_tile_kernel(Operand<T> P,
           for (int k = 0; k < 4; k++) v[k] = acc[i][j][k];
         }
         const int64_t q = q0 + wq + 16 * j + (lane & 15);
-        if (!in_p || q >= Q.rows) continue;
-        if constexpr (MODE == PARTIAL) {
-          *(f32x4*)(e.rows + ((int64_t)split * Q.rows + q) * P.rows + p) = f32x4{v[0], v[1], v[2], v[3]};
+        if (p >= cols || q >= Q.rows) continue;
+        auto value = [&](int k, float x) {                   // x: the residual or dy
+          if constexpr (MODE == FWD) return act_value<ACT>(v[k] + bias[k]) + x;
+          if constexpr (MODE == DZ) {
+            const float d = x * act_slope<ACT>(v[k] + bias[k]);
+            cs[k] += d;
+            return d;
+          }
+          return v[k];
+        };
+        if constexpr (WIDE) {
+          if constexpr (MODE == PARTIAL) {
+            *(f32x4*)(e.rows + ((int64_t)split * Q.rows + q) * P.rows + p) = f32x4{v[0], v[1], v[2], v[3]};
+          } else {
+            Pack<T> o, x;
+#pragma unroll
+            for (int k = 0; k < NV; k++) x.v[k] = 0.f;
+            if constexpr (MODE == FWD)
+              if (e.other) x.load(e.other + q * e.ld + p);
+            if constexpr (MODE == DZ) x.load(e.other + q * e.ld + p);
+#pragma unroll
+            for (int k = 0; k < NV; k++) o.v[k] = value(k, x.v[k]);
+            o.store(e.out + q * e.ld_out + p);
+          }
         } else {
-          Pack<T> o, x;
-          if constexpr (MODE == FWD)
-            if (e.other) x.load(e.other + q * e.ld + p);
-          if constexpr (MODE == DZ) x.load(e.other + q * e.ld + p);
 #pragma unroll
           for (int k = 0; k < NV; k++) {
-            o.v[k] = v[k];
-            if constexpr (MODE == FWD) o.v[k] = act_value<ACT>(v[k] + bias[k]) + (e.other ? x.v[k] : 0.f);
-            if constexpr (MODE == DZ) {
-              o.v[k] = x.v[k] * act_slope<ACT>(v[k] + bias[k]);
-              cs[k] += o.v[k];
+            if (p + k >= cols) continue;
+            const bool in = p + k < P.rows;
+            if constexpr (MODE == PARTIAL) {
+              e.rows[((int64_t)split * Q.rows + q) * P.rows + p + k] = v[k];
+            } else {
+              float x = 0.f;
+              if constexpr (MODE == FWD || MODE == DZ)
+                if (e.other && in) x = to_f32(e.other[q * e.ld + p + k]);
+              e.out[q * e.ld_out + p + k] = in ? from_f32<T>(value(k, x)) : (T)0.f;
             }
           }
-          o.store(e.out + q * P.rows + p);
         }
       }
       if constexpr (MODE == DZ) {
-          float* colsum = (float*)lds;                        // [WQ][TP], the stages are done
+        float* colsum = (float*)lds;                         // [WQ][TP]; the stages are done
 #pragma unroll
         for (int k = 0; k < NV; k++) {
           const float s = row16_sum(cs[k]);
@@ -412,19 +435,23 @@ __global__ __launch_bounds__(256) void lin_any_kernel(Operand<T> P, Operand<T> Q
 #pragma unroll
         for (int r = 0; r < 4; r++) {
           const int p = p0 + wp + i * 16 + (lane >> 4) * 4 + r;
-          if (q >= Q.rows || p >= P.rows) continue;
+          if (q >= Q.rows || p >= (MODE == PARTIAL ? P.rows : e.cols)) continue;
           float v = acc[i][j][r];
-          if constexpr (MODE == FWD || MODE == DZ) v += e.bias ? e.bias[p] : 0.f;
-          if constexpr (MODE == FWD) {
-            v = act_value<ACT>(v);
-            if (e.other) v += to_f32(e.other[q * e.ld + p]);
-          }
-          if constexpr (MODE == DZ) {
-            v = to_f32(e.other[q * e.ld + p]) * act_slope<ACT>(v);
-            cs[i][r] += v;
+          if (p >= P.rows) {
+            v = 0.f;
+          } else {
+            if constexpr (MODE == FWD || MODE == DZ) v += e.bias ? e.bias[p] : 0.f;
+            if constexpr (MODE == FWD) {
+              v = act_value<ACT>(v);
+              if (e.other) v += to_f32(e.other[q * e.ld + p]);
+            }
+            if constexpr (MODE == DZ) {
+              v = to_f32(e.other[q * e.ld + p]) * act_slope<ACT>(v);
+              cs[i][r] += v;
+            }
           }
           if constexpr (MODE == PARTIAL) e.rows[((int64_t)blockIdx.y * Q.rows + q) * P.rows + p] = v;
-          else e.out[q * P.rows + p] = from_f32<T>(v);
+          else e.out[q * e.ld_out + p] = from_f32<T>(v);
         }
       }
     }
@@ -453,7 +480,7 @@ __global__ __launch_bounds__(FEW ? 256 : 1024) void lin_join_kernel(const float*
                                                                     int rows_per_block, Epilogue<T> e) {
   constexpr int LANES = FEW ? 4 : 16;
   __shared__ float red[LANES][64];
-  const int p_blocks = (P + 63) / 64, q_block = blockIdx.x / p_blocks, c = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int p_blocks = (e.cols + 63) / 64, q_block = blockIdx.x / p_blocks, c = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int p = (blockIdx.x - q_block * p_blocks) * 64 + c;
   const int64_t n = (int64_t)P * Q;
   const int qa = q_block * rows_per_block, qb = min(qa + rows_per_block, Q);
@@ -471,8 +498,10 @@ __global__ __launch_bounds__(FEW ? 256 : 1024) void lin_join_kernel(const float*
         v = to_f32(e.other[q * e.ld + p]) * act_slope<ACT>(v + bias);
         cs += v;
       }
-      e.out[(int64_t)q * P + p] = from_f32<T>(v);
+      e.out[q * e.ld_out + p] = from_f32<T>(v);
     };
+    if (!in && p < e.cols)
+      for (int q = qa + w; q < qb; q += LANES) e.out[q * e.ld_out + p] = (T)0.f;
     if constexpr (FEW) {
       if (in)
         for (int q = qa + w; q < qb; q += LANES) {
@@ -511,6 +540,23 @@ __global__ __launch_bounds__(FEW ? 256 : 1024) void lin_join_kernel(const float*
   }
 }
 
+// dst [rows][ld_dst] = src [rows][cols] with zeros behind each row, 16 bytes a thread: operands whose rows are not whole
+// 16-byte chunks are brought into that form once a call.
+template <typename T>
+__global__ __launch_bounds__(256) void lin_pad_kernel(const T* __restrict__ src, int64_t ld, int64_t rows, int cols, int ld_dst,
+                                                      T* __restrict__ dst) {
+  constexpr int V = 16 / sizeof(T);
+  const int per_row = ld_dst / V;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per_row; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per_row;
+    const int c = (int)(i - r * per_row) * V;
+    union { u32x4 u; T t[V]; } x;
+#pragma unroll
+    for (int k = 0; k < V; k++) x.t[k] = c + k < cols ? src[r * ld + c + k] : (T)0.f;
+    *(u32x4*)(dst + r * ld_dst + c) = x.u;
+  }
+}
+
 // rows[chunk][N] = sums of a chunk's rows of d (row stride ld)
 constexpr int SUM_ROWS = 256;
 template <typename T>
@@ -538,6 +584,7 @@ struct Cut {
   Tile tile;
   int splits;
   int64_t per;          // r per split, a multiple of a stage
+  double us;            // the model's time
   int row_tiles() const { return splits > 1 ? JOIN_Q : tile_edge(tile); }      // q rows behind a row of partial sums
 };
 
@@ -548,11 +595,10 @@ struct Cut {
 // each measured in all cuts: the choice is 2 % slower than the best cut on average, 30 % at worst (a 20 us product).
 Cut pick_cut(int esize, bool staged, int64_t p, int64_t q, int64_t r) {
   struct Rate { double full, alone; int at_a_time; };
-  static const Rate rates[] = {{1.5, 1.5, 3}, {0.185, 0.46, 3}, {0.50, 0.90, 2}, {2.0, 0.90, 1}};      // by Tile
+  static const Rate rates[] = {{0.8, 1.2, 3}, {0.185, 0.46, 3}, {0.50, 0.90, 2}, {2.0, 0.90, 1}};      // by Tile
   const int K = ROW_BYTES / esize;
   const int64_t stages = (r + K - 1) / K;
-  Cut best{ANY64, 1, stages * K};
-  double least = 1e300;
+  Cut best{ANY64, 1, stages * K, 1e300};
   for (int t = staged ? T64 : ANY64; t <= (staged ? T256 : ANY64); t++) {
     const int edge = tile_edge((Tile)t), slots = 256 * rates[t].at_a_time;
     const int64_t tiles = (int64_t)cdiv(p, edge) * cdiv(q, edge);
@@ -567,30 +613,26 @@ Cut pick_cut(int esize, bool staged, int64_t p, int64_t q, int64_t r) {
       const int64_t wgs = tiles * splits, rounds = (wgs + slots - 1) / slots;
       double us = (rounds - 1) * round_us(slots, per) + round_us(wgs - (rounds - 1) * slots, per);
       if (splits > 1) us += 2.9 + 3.1e-6 * splits * p * q;
-      if (us < least) {
-        least = us;
-        best = Cut{(Tile)t, splits, per * K};
-      }
+      if (us < best.us) best = Cut{(Tile)t, splits, per * K, us};
     }
   }
   return best;
 }
 
-// Whether the staged kernels take these: everything in 16-byte chunks.
-template <typename T> bool chunked(const Operand<T>& o, int64_t R) {
+// Whether a tensor [..][cols] with this row stride is whole 16-byte chunks, as the staged kernels read it.
+template <typename T> bool chunked(const T* p, int64_t cols, int64_t ld) {
   constexpr int V = 16 / sizeof(T);
-  if ((uintptr_t)o.p & 15) return false;
-  if (o.s_k == 1) return R % V == 0 && o.s_row % V == 0 && o.s_row * (int64_t)sizeof(T) * 256 < 0x7FFFFF00;
-  return o.rows % V == 0 && o.s_k % V == 0 && o.s_k * (int64_t)sizeof(T) * 64 < 0x7FFFFF00;
+  return ((uintptr_t)p & 15) == 0 && cols % V == 0 && ld % V == 0 && ld * (int64_t)sizeof(T) * 256 < 0x7FFFFF00;
 }
 
-template <typename T> bool staged(const Operand<T>& P, const Operand<T>& Q, int64_t R, const Epilogue<T>& e) {
+template <typename T> bool wide_epilogue(const Operand<T>& P, const Epilogue<T>& e, int mode) {
   constexpr int V = 16 / sizeof(T);
-  return chunked(P, R) && chunked(Q, R) && P.rows % V == 0 && (((uintptr_t)e.other | (uintptr_t)e.out) & 15) == 0 &&
+  if (mode == PARTIAL) return P.rows % 4 == 0;
+  return e.cols == P.rows && P.rows % V == 0 && e.ld_out % V == 0 && (((uintptr_t)e.other | (uintptr_t)e.out) & 15) == 0 &&
          (!e.other || e.ld % V == 0);
 }
 
-template <typename T, int TP, int TQ, int WP, int WQ, int STAGES, bool PTR, bool QTR, int MODE>
+template <typename T, int TP, int TQ, int WP, int WQ, int STAGES, bool PTR, bool QTR, int MODE, bool WIDE>
 int launch_tile(const Operand<T>& P, const Operand<T>& Q, int64_t R, const Cut& cut, const Epilogue<T>& e, hipStream_t st) {
   constexpr int LDS = STAGES * (TP + TQ) * ROW_BYTES;
   if constexpr (LDS > 65536) {
@@ -598,23 +640,30 @@ int launch_tile(const Operand<T>& P, const Operand<T>& Q, int64_t R, const Cut& 
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev >= 64) return 1;
     if (!raised[dev]) {
-      if (hipFuncSetAttribute((const void*)lin_tile_kernel<T, TP, TQ, WP, WQ, STAGES, PTR, QTR, MODE>,
+      if (hipFuncSetAttribute((const void*)lin_tile_kernel<T, TP, TQ, WP, WQ, STAGES, PTR, QTR, MODE, WIDE>,
                               hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
         return 1;
       raised[dev] = true;
     }
   }
   const Grid g{cdiv(P.rows, TP), cdiv(Q.rows, TQ), cut.splits, cut.per};
-  lin_tile_kernel<T, TP, TQ, WP, WQ, STAGES, PTR, QTR, MODE><<<g.launch(), 64 * WP * WQ, LDS, st>>>(P, Q, R, g, e);
+  lin_tile_kernel<T, TP, TQ, WP, WQ, STAGES, PTR, QTR, MODE, WIDE><<<g.launch(), 64 * WP * WQ, LDS, st>>>(P, Q, R, g, e);
   return 0;
+}
+
+template <typename T, bool PTR, bool QTR, int MODE, bool WIDE>
+int launch_staged(const Operand<T>& P, const Operand<T>& Q, int64_t R, const Cut& cut, const Epilogue<T>& e, hipStream_t st) {
+  if (cut.tile == T256) return launch_tile<T, 256, 256, 2, 4, 2, PTR, QTR, MODE, WIDE>(P, Q, R, cut, e, st);
+  if (cut.tile == T128) return launch_tile<T, 128, 128, 2, 2, 2, PTR, QTR, MODE, WIDE>(P, Q, R, cut, e, st);
+  return launch_tile<T, 64, 64, 2, 2, 4, PTR, QTR, MODE, WIDE>(P, Q, R, cut, e, st);
 }
 
 template <typename T, bool PTR, bool QTR, int MODE>
 int launch_cut(const Operand<T>& P, const Operand<T>& Q, int64_t R, const Cut& cut, const Epilogue<T>& e, hipStream_t st) {
   switch (cut.tile) {
-    case T256: return launch_tile<T, 256, 256, 2, 4, 2, PTR, QTR, MODE>(P, Q, R, cut, e, st);
-    case T128: return launch_tile<T, 128, 128, 2, 2, 2, PTR, QTR, MODE>(P, Q, R, cut, e, st);
-    case T64: return launch_tile<T, 64, 64, 2, 2, 4, PTR, QTR, MODE>(P, Q, R, cut, e, st);
+    case T256: case T128: case T64:
+      return wide_epilogue(P, e, MODE) ? launch_staged<T, PTR, QTR, MODE, true>(P, Q, R, cut, e, st)
+                                       : launch_staged<T, PTR, QTR, MODE, false>(P, Q, R, cut, e, st);
     default:
       lin_any_kernel<T, MODE><<<dim3(cdiv(P.rows, ANY_T) * cdiv(Q.rows, ANY_T), cut.splits), 256, 0, st>>>(P, Q, R, cut.per, e);
       return 0;
@@ -625,41 +674,68 @@ int launch_cut(const Operand<T>& P, const Operand<T>& Q, int64_t R, const Cut& c
 template <typename T, bool PTR, bool QTR, int MODE>
 int product(const Operand<T>& P, const Operand<T>& Q, int64_t R, const Cut& cut, Epilogue<T> e, float* part, hipStream_t st) {
   if (cut.splits == 1) return launch_cut<T, PTR, QTR, MODE>(P, Q, R, cut, e, st);
-  const Epilogue<T> partial{nullptr, nullptr, 0, nullptr, part, MIS_ACT_NONE};
+  const Epilogue<T> partial{nullptr, nullptr, 0, nullptr, 0, 0, part, MIS_ACT_NONE};
   if (launch_cut<T, PTR, QTR, PARTIAL>(P, Q, R, cut, partial, st)) return 1;
-  const int rpb = MODE == DZ ? JOIN_Q : cut.splits <= JOIN_FEW ? 4 : 1, grid = cdiv(P.rows, 64) * cdiv(Q.rows, rpb);
+  const int rpb = MODE == DZ ? JOIN_Q : cut.splits <= JOIN_FEW ? 4 : 1, grid = cdiv(e.cols, 64) * cdiv(Q.rows, rpb);
   if (cut.splits <= JOIN_FEW) lin_join_kernel<T, MODE, true><<<grid, 256, 0, st>>>(part, cut.splits, P.rows, Q.rows, rpb, e);
   else lin_join_kernel<T, MODE, false><<<grid, 1024, 0, st>>>(part, cut.splits, P.rows, Q.rows, rpb, e);
   return 0;
 }
 
-// Sizes of a call's scratch.  Whether a product can be staged depends on addresses and strides that the size query does
-// not know: the larger of both ways counts.
-size_t part_bytes(int esize, int64_t p, int64_t q, int64_t r) {
+// Scratch of one call, handed out in order; with base 0 the same calls add up its size.
+struct Scratch {
+  uintptr_t base;
+  size_t used;
+  template <typename T> T* take(size_t n) {
+    T* p = (T*)(base + used);
+    used += align256(n * sizeof(T));
+    return p;
+  }
+};
+
+template <typename T> int64_t padded(int64_t n) {
+  constexpr int V = 16 / sizeof(T);
+  return (n + V - 1) / V * V;
+}
+
+// Parts of a split sum, whichever kernel takes it (that depends on addresses the size query does not know).
+size_t part_floats(int esize, int64_t p, int64_t q, int64_t r) {
   size_t most = 0;
   for (int staged = 0; staged < 2; staged++) {
     const Cut c = pick_cut(esize, staged, p, q, r);
-    const size_t n = c.splits > 1 ? (size_t)c.splits * p * q * sizeof(float) : 0;
-    if (n > most) most = n;
+    if (c.splits > 1 && (size_t)c.splits * p * q > most) most = (size_t)c.splits * p * q;
   }
-  return align256(most);
+  return most;
 }
 
-struct BwdPlan {
-  size_t dz, rows, part, total;
+// A copy with padded rows costs a launch and its bytes.
+double pad_us(int64_t rows, int64_t cols, int esize) { return 3.0 + 5e-7 * rows * cols * esize; }
+
+template <typename T>
+const T* pad(const T* src, int64_t rows, int64_t cols, int64_t ld, T* dst, hipStream_t st) {
+  const int64_t ld_dst = padded<T>(cols);
+  lin_pad_kernel<T><<<ew_grid(rows * ld_dst / (16 / (int)sizeof(T)), 256), 256, 0, st>>>(src, ld, rows, (int)cols, (int)ld_dst, dst);
+  return dst;
+}
+
+// The buffers of a call, in the order the code below uses them.  Rows that are not whole 16-byte chunks get a padded copy
+// where that pays; sizes are for the case that it does.
+template <typename T> struct Buffers {
+  T *x, *w, *z;
+  float *rows, *part;
+  Buffers(Scratch& s, int64_t M, int64_t N, int64_t K, int act, bool backward) {
+    const int64_t Kp = padded<T>(K), Np = padded<T>(N);
+    x = s.take<T>(Kp != K ? M * Kp : 0);
+    w = s.take<T>(Kp != K ? N * Kp : 0);
+    z = s.take<T>(!backward ? 0 : act != MIS_ACT_NONE || Np != N ? M * Np : 0);       // dz, or a padded dy
+    size_t most = part_floats(sizeof(T), N, M, K), few_rows = most ? JOIN_Q : 64;
+    rows = s.take<float>(!backward ? 0 : act == MIS_ACT_NONE ? (size_t)cdiv(M, SUM_ROWS) * N : (M + few_rows - 1) / few_rows * N);
+    if (backward)
+      for (size_t n : {part_floats(sizeof(T), K, M, N), part_floats(sizeof(T), K, N, M)})
+        if (n > most) most = n;
+    part = s.take<float>(most);
+  }
 };
-
-BwdPlan bwd_plan(int dtype, int64_t M, int64_t N, int64_t K, int act) {
-  BwdPlan p;
-  const int es = dtype == MIS_BF16 ? 2 : 4;
-  p.dz = act == MIS_ACT_NONE ? 0 : align256((size_t)M * N * es);
-  p.rows = align256((size_t)(act == MIS_ACT_NONE ? cdiv(M, SUM_ROWS) : cdiv(M, pick_cut(es, false, N, M, K).splits > 1 || pick_cut(es, true, N, M, K).splits > 1 ? JOIN_Q : 64)) * N * sizeof(float));
-  p.part = part_bytes(es, K, M, N);
-  for (size_t n : {part_bytes(es, K, N, M), act == MIS_ACT_NONE ? (size_t)0 : part_bytes(es, N, M, K)})
-    if (n > p.part) p.part = n;
-  p.total = p.dz + p.rows + p.part;
-  return p;
-}
 
 bool sizes_ok(int dtype, int64_t M, int64_t N, int64_t K) {
   return (dtype == MIS_F32 || dtype == MIS_BF16) && M >= 1 && N >= 1 && K >= 1 && N <= 1 << 20 && K <= 1 << 20 &&
@@ -674,44 +750,85 @@ bool aligned(int dtype, std::initializer_list<const void*> ps) {
 
 template <typename T>
 int forward(const T* x, int64_t ldx, const T* w, const float* bias, const T* r, int64_t ldr, int64_t M, int64_t N, int64_t K,
-            int act, T* y, char* ws, hipStream_t st) {
-  const Operand<T> P{w, K, 1, (int)N}, Q{x, ldx, 1, (int)M};
-  const Epilogue<T> e{bias, r, ldr, y, nullptr, act};
-  return product<T, false, false, FWD>(P, Q, K, pick_cut(sizeof(T), staged(P, Q, K, e), N, M, K), e, (float*)ws, st);
+            int act, T* y, void* ws, hipStream_t st) {
+  Scratch scratch{(uintptr_t)ws, 0};
+  const Buffers<T> buf(scratch, M, N, K, act, false);
+  const Cut any = pick_cut(sizeof(T), false, N, M, K), fast = pick_cut(sizeof(T), true, N, M, K);
+  int64_t ldw = K;
+  bool staged = chunked(x, K, ldx) && chunked(w, K, ldw);
+  if (padded<T>(K) != K && fast.us + pad_us(M, K, sizeof(T)) + pad_us(N, K, sizeof(T)) < any.us) {
+    x = pad(x, M, K, ldx, buf.x, st);
+    w = pad(w, N, K, ldw, buf.w, st);
+    ldx = ldw = padded<T>(K);
+    staged = true;
+  }
+  const Epilogue<T> e{bias, r, ldr, y, N, (int)N, nullptr, act};
+  return product<T, false, false, FWD>({w, ldw, 1, (int)N}, {x, ldx, 1, (int)M}, K, staged ? fast : any, e, buf.part, st);
 }
 
 template <typename T>
-int backward(const T* x, int64_t ldx, const T* w, const float* bias, const T* dy, int64_t ldd, int dtype, int64_t M, int64_t N,
-             int64_t K, int act, T* dx, T* dw, float* db, char* ws, hipStream_t st) {
-  const BwdPlan p = bwd_plan(dtype, M, N, K, act);
-  T* dz = (T*)ws;
-  float* rows = (float*)(ws + p.dz);
-  float* part = (float*)(ws + p.dz + p.rows);
+int backward(const T* x, int64_t ldx, const T* w, const float* bias, const T* dy, int64_t ldd, int64_t M, int64_t N, int64_t K,
+             int act, T* dx, T* dw, float* db, void* ws, hipStream_t st) {
+  Scratch scratch{(uintptr_t)ws, 0};
+  const Buffers<T> buf(scratch, M, N, K, act, true);
+  const bool again = act != MIS_ACT_NONE;
+  const int64_t Kp = padded<T>(K), Np = padded<T>(N);
+  Cut dz_cut[2], dx_cut[2], dw_cut[2];                   // [staged]
+  double us[2] = {0.0, 0.0};
+  for (int i = 0; i < 2; i++) {
+    dz_cut[i] = pick_cut(sizeof(T), i, N, M, K);
+    dx_cut[i] = pick_cut(sizeof(T), i, K, M, N);
+    dw_cut[i] = pick_cut(sizeof(T), i, K, N, M);
+    us[i] = (again ? dz_cut[i].us : 0.0) + (dx ? dx_cut[i].us : 0.0) + (dw ? dw_cut[i].us : 0.0);
+  }
+  const bool pad_k = Kp != K, pad_dy = Np != N && !again;
+  const bool use_x = again || dw, use_w = again || dx;
+  int64_t ldw = K;
+  bool staged = (pad_k || ((!use_x || chunked(x, K, ldx)) && (!use_w || chunked(w, K, ldw)))) &&
+                (again || pad_dy || chunked(dy, N, ldd));
+  if (staged && (pad_k || pad_dy)) {
+    double extra = 0.0;
+    if (pad_k) extra += (use_x ? pad_us(M, K, sizeof(T)) : 0.0) + (use_w ? pad_us(N, K, sizeof(T)) : 0.0);
+    if (pad_dy) extra += pad_us(M, N, sizeof(T));
+    staged = us[1] + extra < us[0];
+    if (staged && pad_k) {
+      if (use_x) x = pad(x, M, K, ldx, buf.x, st);
+      if (use_w) w = pad(w, N, K, ldw, buf.w, st);
+      ldx = ldw = Kp;
+    }
+  }
   const T* z = dy;
   int64_t ldz = ldd;
-  if (act != MIS_ACT_NONE) {
-    const Operand<T> P{w, K, 1, (int)N}, Q{x, ldx, 1, (int)M};
-    const Epilogue<T> e{bias, dy, ldd, dz, rows, act};
-    const Cut cut = pick_cut(sizeof(T), staged(P, Q, K, e), N, M, K);
-    if (product<T, false, false, DZ>(P, Q, K, cut, e, part, st)) return 1;
-    z = dz;
-    ldz = N;
-    if (db) launch_reduce_partials(rows, cdiv(M, cut.row_tiles()), (int)N, db, st);
+  if (again) {
+    const Epilogue<T> e{bias, dy, ldd, buf.z, Np, (int)Np, buf.rows, act};
+    const Cut& cut = dz_cut[staged];
+    if (product<T, false, false, DZ>({w, ldw, 1, (int)N}, {x, ldx, 1, (int)M}, K, cut, e, buf.part, st)) return 1;
+    z = buf.z;
+    ldz = Np;
+    if (db) launch_reduce_partials(buf.rows, cdiv(M, cut.row_tiles()), (int)N, db, st);
   } else if (db) {
-    lin_colsum_kernel<T><<<dim3(cdiv(M, SUM_ROWS), cdiv(N, 64)), 256, 0, st>>>(dy, ldd, M, (int)N, rows);
-    launch_reduce_partials(rows, cdiv(M, SUM_ROWS), (int)N, db, st);
+    lin_colsum_kernel<T><<<dim3(cdiv(M, SUM_ROWS), cdiv(N, 64)), 256, 0, st>>>(dy, ldd, M, (int)N, buf.rows);
+    launch_reduce_partials(buf.rows, cdiv(M, SUM_ROWS), (int)N, db, st);
+  }
+  if (staged && pad_dy && (dx || dw)) {
+    z = pad(dy, M, N, ldd, buf.z, st);
+    ldz = Np;
   }
   if (dx) {
-    const Operand<T> P{w, 1, K, (int)K}, Q{z, ldz, 1, (int)M};
-    const Epilogue<T> e{nullptr, nullptr, 0, dx, nullptr, MIS_ACT_NONE};
-    if (product<T, true, false, STORE>(P, Q, N, pick_cut(sizeof(T), staged(P, Q, N, e), K, M, N), e, part, st)) return 1;
+    const Epilogue<T> e{nullptr, nullptr, 0, dx, K, (int)K, nullptr, MIS_ACT_NONE};
+    if (product<T, true, false, STORE>({w, 1, ldw, (int)K}, {z, ldz, 1, (int)M}, N, dx_cut[staged], e, buf.part, st)) return 1;
   }
   if (dw) {
-    const Operand<T> P{x, 1, ldx, (int)K}, Q{z, 1, ldz, (int)N};
-    const Epilogue<T> e{nullptr, nullptr, 0, dw, nullptr, MIS_ACT_NONE};
-    if (product<T, true, true, STORE>(P, Q, M, pick_cut(sizeof(T), staged(P, Q, M, e), K, N, M), e, part, st)) return 1;
+    const Epilogue<T> e{nullptr, nullptr, 0, dw, K, (int)K, nullptr, MIS_ACT_NONE};
+    if (product<T, true, true, STORE>({x, 1, ldx, (int)K}, {z, 1, ldz, (int)N}, M, dw_cut[staged], e, buf.part, st)) return 1;
   }
   return 0;
+}
+
+template <typename T> size_t bytes_of(int64_t M, int64_t N, int64_t K, int act, bool backward) {
+  Scratch s{0, 0};
+  Buffers<T>(s, M, N, K, act, backward);
+  return s.used ? s.used : 256;
 }
 
 }  // namespace
@@ -720,8 +837,7 @@ extern "C" {
 
 size_t mis_linear_act_fwd_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
   if (!sizes_ok(dtype, M, N, K)) return 0;
-  const size_t n = part_bytes(dtype == MIS_BF16 ? 2 : 4, N, M, K);
-  return n ? n : 256;
+  return dtype == MIS_BF16 ? bytes_of<bf16>(M, N, K, MIS_ACT_NONE, false) : bytes_of<float>(M, N, K, MIS_ACT_NONE, false);
 }
 
 int mis_linear_act_fwd(const void* x, int64_t ldx, const void* w, const float* bias, const void* residual, int64_t ldr, int dtype,
@@ -736,17 +852,18 @@ int mis_linear_act_fwd(const void* x, int64_t ldx, const void* w, const float* b
   int rc;
   if (dtype == MIS_BF16)
     rc = forward((const bf16*)x, ldx, (const bf16*)w, bias, (const bf16*)residual, ldr, M, N, K, act, (bf16*)y,
-                 (char*)workspace, st);
+                 workspace, st);
   else
     rc = forward((const float*)x, ldx, (const float*)w, bias, (const float*)residual, ldr, M, N, K, act, (float*)y,
-                 (char*)workspace, st);
+                 workspace, st);
   MIS_REQUIRE(rc == 0, "linear_act_fwd: the device refuses the kernel's shared memory");
   MIS_CHECK_LAUNCH("linear_act_fwd");
   return MIS_OK;
 }
 
 size_t mis_linear_act_bwd_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K, int act) {
-  return sizes_ok(dtype, M, N, K) ? bwd_plan(dtype, M, N, K, act).total : 0;
+  if (!sizes_ok(dtype, M, N, K)) return 0;
+  return dtype == MIS_BF16 ? bytes_of<bf16>(M, N, K, act, true) : bytes_of<float>(M, N, K, act, true);
 }
 
 int mis_linear_act_bwd(const void* x, int64_t ldx, const void* w, const float* bias, const void* dy, int64_t ldd, int dtype,
@@ -761,11 +878,11 @@ int mis_linear_act_bwd(const void* x, int64_t ldx, const void* w, const float* b
   hipStream_t st = (hipStream_t)stream;
   int rc;
   if (dtype == MIS_BF16)
-    rc = backward((const bf16*)x, ldx, (const bf16*)w, bias, (const bf16*)dy, ldd, dtype, M, N, K, act, (bf16*)dx, (bf16*)dw, db,
-             (char*)workspace, st);
+    rc = backward((const bf16*)x, ldx, (const bf16*)w, bias, (const bf16*)dy, ldd, M, N, K, act, (bf16*)dx, (bf16*)dw, db,
+             workspace, st);
   else
-    rc = backward((const float*)x, ldx, (const float*)w, bias, (const float*)dy, ldd, dtype, M, N, K, act, (float*)dx, (float*)dw, db,
-             (char*)workspace, st);
+    rc = backward((const float*)x, ldx, (const float*)w, bias, (const float*)dy, ldd, M, N, K, act, (float*)dx, (float*)dw, db,
+             workspace, st);
   MIS_REQUIRE(rc == 0, "linear_act_bwd: the device refuses the kernel's shared memory");
   MIS_CHECK_LAUNCH("linear_act_bwd");
   return MIS_OK;
