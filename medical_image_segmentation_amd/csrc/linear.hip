@@ -214,6 +214,7 @@ template <typename T, int TP, int TQ, int WP, int WQ, int STAGES, bool PTR, bool
 __global__ __launch_bounds__(64 * WP * WQ, 2) void lin_tile_kernel(Operand<T> P, Operand<T> Q, int64_t R, Grid grid,
                                                                    Epilogue<T> e) {
   constexpr int THREADS = 64 * WP * WQ, BP = TP / WP / 16, BQ = TQ / WQ / 16, K = ROW_BYTES / (int)sizeof(T);
+  static_assert(BP >= BQ, "the second half's fragments of both operands are read in BP steps");
   constexpr int STAGE = (TP + TQ) * ROW_BYTES;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
@@ -254,18 +255,26 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void lin_tile_kernel(Operand<T> P,
     load(cur == 0 ? STAGES - 1 : cur - 1);
     const char* tp = lds + cur * STAGE;
     const char* tq = tp + TP * ROW_BYTES;
+    // The second half's fragments are read between the products of the first: the compiler on its own reads each just
+    // before its use (8192x4096->4096 forward and its two backward products 238, 265, 247 -> 232, 247, 234 us).
+    u32x4 a[2][BP], b[2][BQ];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      u32x4 a[BP], b[BQ];
+    for (int j = 0; j < BQ; j++) b[0][j] = fragment<T, TQ, QTR>(tq, wq + 16 * j, 0);
 #pragma unroll
-      for (int i = 0; i < BP; i++) a[i] = fragment<T, TP, PTR>(tp, wp + 16 * i, h);
+    for (int i = 0; i < BP; i++) a[0][i] = fragment<T, TP, PTR>(tp, wp + 16 * i, 0);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int j = 0; j < BQ; j++) b[j] = fragment<T, TQ, QTR>(tq, wq + 16 * j, h);
+    for (int i = 0; i < BP; i++) {
 #pragma unroll
-      for (int i = 0; i < BP; i++)
-#pragma unroll
-        for (int j = 0; j < BQ; j++) acc[i][j] = multiply(a[i], b[j], acc[i][j], T());
+      for (int j = 0; j < BQ; j++) acc[i][j] = multiply(a[0][i], b[0][j], acc[i][j], T());
+      a[1][i] = fragment<T, TP, PTR>(tp, wp + 16 * i, 1);
+      if (i < BQ) b[1][i] = fragment<T, TQ, QTR>(tq, wq + 16 * i, 1);
+      __builtin_amdgcn_sched_barrier(0);
     }
+#pragma unroll
+    for (int i = 0; i < BP; i++)
+#pragma unroll
+      for (int j = 0; j < BQ; j++) acc[i][j] = multiply(a[1][i], b[1][j], acc[i][j], T());
     cur = cur + 1 == STAGES ? 0 : cur + 1;
   }
   wait_and_meet<0>();                       // (no load may reach LDS that this workgroup no longer owns)
