@@ -18,6 +18,9 @@
 //
 // HBM-bound: parameter read and written, gradient read (twice when clipping: the norm comes first), four code bytes
 // and a 64th of that in scales per element: 16 (20) bytes per float32 element against 28 (32) with float32 moments.
+// At that rate the vector units have about 100 instruction slots per element, so their number is kept down: codes are
+// decoded by a table of doubles in LDS, exclusive-ors are three-operand, blocks whose values are too small or not finite
+// take a slow way of their own, and a workgroup walks neighbouring chunks with the next one's loads under way.
 #include "common.h"
 
 namespace {
@@ -25,6 +28,7 @@ namespace {
 constexpr int A8_THREADS = 256;
 constexpr int A8_CHUNK = 4096;        // MIS_OPT_CHUNK
 constexpr int A8_PARTIALS = 1024;     // partial sums of the norm: few enough for every workgroup to add up
+constexpr int A8_GRID = 2048;         // most workgroups of a step: what the chip holds at once, each with a run of chunks
 
 struct Desc8 {
   void* p;
@@ -66,25 +70,6 @@ __device__ __forceinline__ double sum_of_block(double v, double* red) {
   return s;
 }
 
-// Eight consecutive elements; those from n on read as zero.
-template <typename T>
-__device__ __forceinline__ void load8(const T* __restrict__ p, int64_t e, int64_t n, bool wide, float (&f)[8]) {
-  if (wide && e + 8 <= n) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = *(const float4*)(p + e), b = *(const float4*)(p + e + 4);
-      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-      f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-    } else {
-      const bf16x8 a = *(const bf16x8*)(p + e);
-#pragma unroll
-      for (int i = 0; i < 8; i++) f[i] = (float)a[i];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) f[i] = e + i < n ? to_f32(p[e + i]) : 0.f;
-  }
-}
-
 template <typename T>
 __device__ __forceinline__ void store8(T* __restrict__ p, int64_t e, int64_t n, bool wide, const float (&f)[8]) {
   if (wide && e + 8 <= n) {
@@ -104,19 +89,65 @@ __device__ __forceinline__ void store8(T* __restrict__ p, int64_t e, int64_t n, 
   }
 }
 
+// Eight consecutive elements as they lie in memory; those from n on as zeros.
+template <typename T> struct Raw8 {
+  static constexpr int W = sizeof(T) / 2;
+  uint4 u[W];
+  __device__ __forceinline__ void load(const T* __restrict__ p, int64_t e, int64_t n, bool wide) {
+    if (wide && e + 8 <= n) {
+#pragma unroll
+      for (int i = 0; i < W; i++) u[i] = ((const uint4*)(p + e))[i];
+    } else {
+      union { uint4 u[W]; T t[8]; } x;
+#pragma unroll
+      for (int i = 0; i < 8; i++) x.t[i] = e + i < n ? p[e + i] : (T)0.f;
+#pragma unroll
+      for (int i = 0; i < W; i++) u[i] = x.u[i];
+    }
+  }
+  __device__ __forceinline__ void floats(float (&f)[8]) const {
+    union { uint4 u[W]; T t[8]; } x;
+#pragma unroll
+    for (int i = 0; i < W; i++) x.u[i] = u[i];
+#pragma unroll
+    for (int i = 0; i < 8; i++) f[i] = to_f32(x.t[i]);
+  }
+};
+
+// A workgroup's run of chunks, and the tensor that the current one lies in.
+struct Walk {
+  const int* prefix;
+  int c, end, t;
+  __device__ __forceinline__ Walk(const int* prefix_, int n_tensors, int first, int n, int wg, int wgs) : prefix(prefix_) {
+    const int per = n / wgs, more = n - per * wgs;       // the first `more` workgroups take one chunk more
+    c = first + wg * per + min(wg, more);
+    end = c + per + (wg < more ? 1 : 0);
+    t = c < end ? tensor_of(prefix, n_tensors, c) : 0;
+  }
+  __device__ __forceinline__ void next() {
+    c++;
+    while (c < end && prefix[t + 1] <= c) t++;
+  }
+};
+
 template <typename T>
 __device__ __forceinline__ double chunk_sqsum(const T* __restrict__ g, int64_t e0, int64_t n) {
+  constexpr int N = A8_CHUNK / (A8_THREADS * 8);
   const bool wide = ((uintptr_t)g & 15) == 0;
+  Raw8<T> r[N];
+#pragma unroll
+  for (int it = 0; it < N; it++) {
+    const int64_t e = e0 + (it * A8_THREADS + threadIdx.x) * 8;
+    if (e < n) r[it].load(g, e, n, wide);
+    else r[it] = Raw8<T>{};
+  }
   double s = 0.0;
 #pragma unroll
-  for (int it = 0; it < A8_CHUNK / (A8_THREADS * 8); it++) {
-    const int64_t e = e0 + (it * A8_THREADS + threadIdx.x) * 8;
-    if (e < n) {
-      float f[8];
-      load8(g, e, n, wide, f);
+  for (int it = 0; it < N; it++) {
+    float f[8];
+    r[it].floats(f);
 #pragma unroll
-      for (int i = 0; i < 8; i++) s = fma((double)f[i], (double)f[i], s);
-    }
+    for (int i = 0; i < 8; i++) s = fma((double)f[i], (double)f[i], s);
   }
   return s;
 }
@@ -126,14 +157,21 @@ __global__ __launch_bounds__(A8_THREADS) void adamw8_sqsum_kernel(const Desc8* _
                                                                   int n_chunks, double* __restrict__ partials) {
   __shared__ double red[A8_THREADS / 64];
   double s = 0.0;
-  for (int c = blockIdx.x; c < n_chunks; c += gridDim.x) {
-    const int t = tensor_of(prefix, n_tensors, c);
-    const Desc8 d = descs[t];
-    const int64_t e0 = (int64_t)(c - prefix[t]) * A8_CHUNK;
+  for (Walk w(prefix, n_tensors, 0, n_chunks, blockIdx.x, gridDim.x); w.c < w.end; w.next()) {
+    const Desc8 d = descs[w.t];
+    const int64_t e0 = (int64_t)(w.c - prefix[w.t]) * A8_CHUNK;
     s += d.dtype == MIS_F32 ? chunk_sqsum((const float*)d.g, e0, d.n) : chunk_sqsum((const bf16*)d.g, e0, d.n);
   }
   s = sum_of_block(s, red);
   if (threadIdx.x == 0) partials[blockIdx.x] = s;
+}
+
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+#ifdef __HIP_DEVICE_COMPILE__
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);
+#else
+  return a ^ b ^ c;
+#endif
 }
 
 // Philox4x32-10: four words for the counter (c0, c1, c2, c3) under the key (k0, k1).
@@ -141,7 +179,7 @@ __device__ __forceinline__ void philox10(uint32_t (&c)[4], uint32_t k0, uint32_t
 #pragma unroll
   for (int r = 0; r < 10; r++) {
     const uint64_t p = (uint64_t)c[0] * 0xD2511F53u, q = (uint64_t)c[2] * 0xCD9E8D57u;
-    const uint32_t n0 = (uint32_t)(q >> 32) ^ c[1] ^ k0, n2 = (uint32_t)(p >> 32) ^ c[3] ^ k1;
+    const uint32_t n0 = xor3((uint32_t)(q >> 32), c[1], k0), n2 = xor3((uint32_t)(p >> 32), c[3], k1);
     c[1] = (uint32_t)q;
     c[3] = (uint32_t)p;
     c[0] = n0;
@@ -186,78 +224,156 @@ __device__ __forceinline__ uint32_t code_of(uint32_t b, int s, uint32_t r) {
   return ((b != 0 && t >= (1 << 23) ? (uint32_t)t : low) + r) >> DROP;
 }
 
+// The same for SAFE <= s < 255 without the special cases: the mantissa is shifted down to the block's linear binade.
+// Zero and numbers below 2^-126 have exponent field 0 and are shifted by at least 24 bits: they give 0 by themselves.
+constexpr uint32_t SAFE = 40;
+template <int DROP>
+__device__ __forceinline__ uint32_t safe_code_of(uint32_t b, uint32_t s, uint32_t r) {
+  const int shift = (int)(s - 14) - (int)(b >> 23);
+  const uint32_t low = ((b & 0x007FFFFFu) | 0x00800000u) >> min(shift, 31);
+  return ((shift > 0 ? low : b - ((s - 15) << 23)) + r) >> DROP;
+}
+
+__device__ __forceinline__ uint32_t bytes4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return a | b << 8 | c << 16 | d << 24;
+}
+
+// What a thread holds of its 8 elements before the update, raw.
+template <typename T> struct Item {
+  Raw8<T> p, g;
+  uint2 m, v;
+  uint32_t sm, sv;
+  int64_t e;              // first element within the tensor; behind the padded tensor: nothing to do
+};
+
+struct Buffers8 {
+  uint8_t *m, *ms, *v, *vs;
+};
+
 template <typename T>
-__device__ __forceinline__ void adamw8_chunk(const Desc8& d, int64_t e0, const Args8& a, const Step8& st, double coef,
-                                             uint8_t* __restrict__ mc, uint8_t* __restrict__ msc, uint8_t* __restrict__ vc,
-                                             uint8_t* __restrict__ vsc) {
-  T* P = (T*)d.p;
-  const T* G = (const T*)d.g;
-  const bool pw = ((uintptr_t)P & 15) == 0, gw = ((uintptr_t)G & 15) == 0;
-  const int64_t padded = (d.n + 127) & ~(int64_t)127;
+__device__ __forceinline__ void fetch(Item<T>& x, const Desc8& d, int64_t e, const Buffers8& b) {
+  x.e = e;
+  if (e >= ((d.n + 127) & ~(int64_t)127)) return;        // (all 16 lanes of a block, or none)
+  const int64_t f = d.off + e;
+  x.g.load((const T*)d.g, e, d.n, ((uintptr_t)d.g & 15) == 0);
+  x.p.load((const T*)d.p, e, d.n, ((uintptr_t)d.p & 15) == 0);
+  x.m = *(const uint2*)(b.m + f);
+  x.v = *(const uint2*)(b.v + f);
+  x.sm = b.ms[f >> 7];
+  x.sv = b.vs[f >> 7];
+}
+
+// c1 = (1-b1) coef, c2 = (1-b2) coef^2; m_table, v_table: what the codes stand for in a block of exponent 127
+template <typename T>
+__device__ __forceinline__ void update(const Item<T>& x, const Desc8& d, const Args8& a, const Step8& st, double c1, double c2,
+                                       const double* m_table, const double* v_table, const Buffers8& buf) {
+  if (x.e >= ((d.n + 127) & ~(int64_t)127)) return;
+  const int64_t f = d.off + x.e;
+  float p[8], g[8];
+  x.p.floats(p);
+  x.g.floats(g);
+  const double fm = a.b1 * block_factor(x.sm), fv = a.b2 * block_factor(x.sv);
+  uint32_t rnd[8];
 #pragma unroll
-  for (int it = 0; it < A8_CHUNK / (A8_THREADS * 8); it++) {
-    const int64_t e = e0 + (it * A8_THREADS + threadIdx.x) * 8;
-    if (e >= padded) continue;                 // (all 16 lanes of a block, or none)
-    const int64_t f = d.off + e;
-    float p[8], g[8];
-    load8(G, e, d.n, gw, g);
-    load8((const T*)P, e, d.n, pw, p);
-    union { uint2 u; uint8_t b[8]; } km, kv;
-    km.u = *(const uint2*)(mc + f);
-    kv.u = *(const uint2*)(vc + f);
-    const double fm = a.b1 * block_factor(msc[f >> 7]), fv = a.b2 * block_factor(vsc[f >> 7]);
-    uint32_t rnd[8];
+  for (int h = 0; h < 2; h++) {
+    const uint64_t q = (uint64_t)(f >> 2) + h;
+    uint32_t c[4] = {(uint32_t)q, (uint32_t)(q >> 32), st.step_lo, st.step_hi};
+    philox10(c, a.seed_lo, a.seed_hi);
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const uint64_t q = (uint64_t)(f >> 2) + h;
-      uint32_t c[4] = {(uint32_t)q, (uint32_t)(q >> 32), st.step_lo, st.step_hi};
-      philox10(c, a.seed_lo, a.seed_hi);
+    for (int i = 0; i < 4; i++) rnd[4 * h + i] = c[i];
+  }
+  float m[8], v[8];
+  uint32_t mb[8], vb[8], mmax = 0, vmax = 0;
 #pragma unroll
-      for (int i = 0; i < 4; i++) rnd[4 * h + i] = c[i];
-    }
-    uint32_t mb[8], vb[8], sign[8], mmax = 0, vmax = 0;
+  for (int i = 0; i < 8; i++) {
+    const uint32_t km = ((i < 4 ? x.m.x : x.m.y) >> 8 * (i & 3)) & 255, kv = ((i < 4 ? x.v.x : x.v.y) >> 8 * (i & 3)) & 255;
+    const double gd = (double)g[i];
+    m[i] = (float)fma(c1, gd, fm * m_table[km]);
+    v[i] = (float)fma(c2, gd * gd, fv * v_table[kv]);
+    const float denom = fmaf(__builtin_amdgcn_sqrtf(v[i]), st.inv_bc2, a.eps);
+    p[i] = fmaf(p[i], st.decay, -st.step_size * (m[i] * __builtin_amdgcn_rcpf(denom)));
+    mb[i] = __builtin_bit_cast(uint32_t, m[i]) & 0x7FFFFFFFu;
+    vb[i] = __builtin_bit_cast(uint32_t, v[i]);
+    mmax = max(mmax, mb[i]);
+    vmax = max(vmax, vb[i]);
+  }
+  store8((T*)d.p, x.e, d.n, ((uintptr_t)d.p & 15) == 0, p);
+  mmax = row16_max(mmax);
+  vmax = row16_max(vmax);
+  uint32_t sm = min((mmax + 0x000FFFFFu) >> 23, 255u), sv = min((vmax + 0x0007FFFFu) >> 23, 255u);
+  uint32_t qm[8], qv[8];
+  if (__builtin_expect(sm - SAFE < 255 - SAFE && sv - SAFE < 255 - SAFE, 1)) {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const double gd = (double)g[i] * coef;
-      const float m = (float)fma(fm, (double)m_code_float(km.b[i]), a.omb1 * gd);
-      const float v = (float)fma(fv, (double)v_code_float(kv.b[i]), a.omb2 * gd * gd);
-      const float denom = fmaf(__builtin_amdgcn_sqrtf(v), st.inv_bc2, a.eps);
-      p[i] = fmaf(p[i], st.decay, -st.step_size * (m * __builtin_amdgcn_rcpf(denom)));
-      mb[i] = mag_bits(m);
-      vb[i] = mag_bits(v);
-      sign[i] = __builtin_bit_cast(uint32_t, m) >> 31;
+      qm[i] = safe_code_of<20>(mb[i], sm, (rnd[i] << 4 & 0xFFFF0u) | 8u);
+      qv[i] = safe_code_of<19>(vb[i], sv, (rnd[i] >> 13 & 0x7FFF8u) | 4u);
+      if (vb[i] >= 0x00800000u) qv[i] = max(qv[i], 1u);
+      qm[i] |= __builtin_bit_cast(uint32_t, m[i]) >> 24 & 0x80u;
+    }
+  } else {                                     // tiny, zero or not finite
+    mmax = vmax = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      mb[i] = mag_bits(m[i]);
+      vb[i] = mag_bits(v[i]);
       mmax = max(mmax, mb[i]);
       vmax = max(vmax, vb[i]);
     }
-    store8(P, e, d.n, pw, p);
-    const uint32_t sm = min((row16_max(mmax) + 0x000FFFFFu) >> 23, 255u);
-    const uint32_t sv = min((row16_max(vmax) + 0x0007FFFFu) >> 23, 255u);
+    sm = min((row16_max(mmax) + 0x000FFFFFu) >> 23, 255u);
+    sv = min((row16_max(vmax) + 0x0007FFFFu) >> 23, 255u);
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const uint32_t qm = code_of<20>(mb[i], (int)sm, (rnd[i] & 0xFFFFu) << 4 | 8u);
-      uint32_t qv = code_of<19>(vb[i], (int)sv, (rnd[i] >> 16) << 3 | 4u);
-      if (qv == 0 && vb[i] != 0) qv = 1;
-      km.b[i] = (uint8_t)((sm == 255 ? 0u : qm) | sign[i] << 7);
-      kv.b[i] = (uint8_t)(sv == 255 ? 0u : qv);
+      qm[i] = sm == 255 ? 0u : code_of<20>(mb[i], (int)sm, (rnd[i] << 4 & 0xFFFF0u) | 8u);
+      qv[i] = sv == 255 ? 0u : code_of<19>(vb[i], (int)sv, (rnd[i] >> 13 & 0x7FFF8u) | 4u);
+      if (qv[i] == 0 && vb[i] != 0 && sv != 255) qv[i] = 1;
+      qm[i] |= __builtin_bit_cast(uint32_t, m[i]) >> 24 & 0x80u;
     }
-    *(uint2*)(mc + f) = km.u;
-    *(uint2*)(vc + f) = kv.u;
-    if ((threadIdx.x & 15) == 0) {
-      msc[f >> 7] = (uint8_t)sm;
-      vsc[f >> 7] = (uint8_t)sv;
-    }
+  }
+  *(uint2*)(buf.m + f) = make_uint2(bytes4(qm[0], qm[1], qm[2], qm[3]), bytes4(qm[4], qm[5], qm[6], qm[7]));
+  *(uint2*)(buf.v + f) = make_uint2(bytes4(qv[0], qv[1], qv[2], qv[3]), bytes4(qv[4], qv[5], qv[6], qv[7]));
+  if ((threadIdx.x & 15) == 0) {
+    buf.ms[f >> 7] = (uint8_t)sm;
+    buf.vs[f >> 7] = (uint8_t)sv;
+  }
+}
+
+// The chunks of a run that lie in tensors of one type: half a chunk at a time, the next half's loads before the update.
+template <typename T>
+__device__ __forceinline__ void adamw8_run(Walk& w, Desc8& d, const Desc8* __restrict__ descs, const Args8& a, const Step8& st,
+                                           double c1, double c2, const double* m_table, const double* v_table,
+                                           const Buffers8& buf) {
+  constexpr int HALF = A8_THREADS * 8;
+  Item<T> x, y;
+  Desc8 dx = d, dy;
+  fetch(x, dx, (int64_t)(w.c - w.prefix[w.t]) * A8_CHUNK + threadIdx.x * 8, buf);
+  while (true) {
+    fetch(y, dx, x.e + HALF, buf);
+    update(x, dx, a, st, c1, c2, m_table, v_table, buf);
+    const int64_t ey = y.e;
+    const int t = w.t;
+    w.next();
+    const bool more = w.c < w.end;
+    dy = dx;
+    if (more && w.t != t) d = dy = descs[w.t];
+    const bool same = more && dy.dtype == dx.dtype;
+    if (same) fetch(x, dy, (int64_t)(w.c - w.prefix[w.t]) * A8_CHUNK + threadIdx.x * 8, buf);
+    update(y, dx, a, st, c1, c2, m_table, v_table, buf);
+    if (!same) return;
+    dx = dy;
   }
 }
 
 __global__ __launch_bounds__(A8_THREADS) void adamw8_step_kernel(const Desc8* __restrict__ descs,
                                                                  const int* __restrict__ prefix, int n_tensors, int chunk0,
-                                                                 Args8 a, const Step8* __restrict__ dyn,
+                                                                 int n_chunks, Args8 a, const Step8* __restrict__ dyn,
                                                                  const double* __restrict__ partials, int n_partials,
-                                                                 uint8_t* __restrict__ mc, uint8_t* __restrict__ msc,
-                                                                 uint8_t* __restrict__ vc, uint8_t* __restrict__ vsc,
-                                                                 float* __restrict__ norm_out) {
-  __shared__ double red[A8_THREADS / 64];
+                                                                 Buffers8 buf, float* __restrict__ norm_out) {
+  __shared__ double red[A8_THREADS / 64], m_table[256], v_table[256];
   const Step8 st = dyn ? *dyn : a.s;
+  for (int k = threadIdx.x; k < 256; k += A8_THREADS) {
+    m_table[k] = (double)m_code_float(k);
+    v_table[k] = (double)v_code_float(k);
+  }
   double coef = 1.0;
   if (partials) {                              // every workgroup: the same sum in the same order
     double s = 0.0;
@@ -267,32 +383,38 @@ __global__ __launch_bounds__(A8_THREADS) void adamw8_step_kernel(const Desc8* __
     if (coef > 1.0) coef = 1.0;                // (NaN stays NaN)
     if (a.max_norm <= 0.0) coef = 1.0;
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = (float)norm;
+  } else {
+    __syncthreads();
   }
-  const int chunk = chunk0 + blockIdx.x;
-  const int t = tensor_of(prefix, n_tensors, chunk);
-  const Desc8 d = descs[t];
-  const int64_t e0 = (int64_t)(chunk - prefix[t]) * A8_CHUNK;
-  if (d.dtype == MIS_F32) adamw8_chunk<float>(d, e0, a, st, coef, mc, msc, vc, vsc);
-  else adamw8_chunk<bf16>(d, e0, a, st, coef, mc, msc, vc, vsc);
+  const double c1 = a.omb1 * coef, c2 = a.omb2 * coef * coef;
+  Walk w(prefix, n_tensors, chunk0, n_chunks, blockIdx.x, gridDim.x);
+  if (w.c >= w.end) return;
+  Desc8 d = descs[w.t];
+  while (w.c < w.end) {
+    if (d.dtype == MIS_F32) adamw8_run<float>(w, d, descs, a, st, c1, c2, m_table, v_table, buf);
+    else adamw8_run<bf16>(w, d, descs, a, st, c1, c2, m_table, v_table, buf);
+  }
 }
 
-// The moments that the codes stand for.
-__global__ __launch_bounds__(A8_THREADS) void adamw8_moments_kernel(const uint8_t* __restrict__ mc, const uint8_t* __restrict__ msc,
-                                                                    const uint8_t* __restrict__ vc, const uint8_t* __restrict__ vsc,
-                                                                    int64_t n8, float* __restrict__ m, float* __restrict__ v) {
-  for (int64_t i = (int64_t)blockIdx.x * A8_THREADS + threadIdx.x; i < n8; i += (int64_t)gridDim.x * A8_THREADS) {
-    union { uint2 u; uint8_t b[8]; } km, kv;
-    km.u = *(const uint2*)(mc + i * 8);
-    kv.u = *(const uint2*)(vc + i * 8);
-    const double fm = block_factor(msc[i >> 4]), fv = block_factor(vsc[i >> 4]);
-    float om[8], ov[8];
+// The moments that the codes stand for: 4 elements a thread at a time.
+__global__ __launch_bounds__(A8_THREADS) void adamw8_moments_kernel(const uint32_t* __restrict__ mc, const uint8_t* __restrict__ msc,
+                                                                    const uint32_t* __restrict__ vc, const uint8_t* __restrict__ vsc,
+                                                                    int64_t n4, float4* __restrict__ m, float4* __restrict__ v) {
+  const int64_t stride = (int64_t)gridDim.x * A8_THREADS;
+#pragma unroll 2
+  for (int64_t i = (int64_t)blockIdx.x * A8_THREADS + threadIdx.x; i < n4; i += stride) {
+    const uint32_t km = mc[i], kv = vc[i];
+    const int sm = msc[i >> 5], sv = vsc[i >> 5];
+    // 2^(s-15) times the code as a float; a factor of NaN or zero for s = 255 and 0
+    const float om = sm == 255 ? __builtin_nanf("") : sm == 0 ? 0.f : 1.f, ov = sv == 255 ? __builtin_nanf("") : sv == 0 ? 0.f : 1.f;
+    float fm[4], fv[4];
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-      om[k] = (float)(fm * (double)m_code_float(km.b[k]));
-      ov[k] = (float)(fv * (double)v_code_float(kv.b[k]));
+    for (int k = 0; k < 4; k++) {
+      fm[k] = om * ldexpf(m_code_float(km >> 8 * k & 255), sm - 15);
+      fv[k] = ov * ldexpf(v_code_float(kv >> 8 * k & 255), sv - 15);
     }
-    store8(m, i * 8, n8 * 8, true, om);
-    store8(v, i * 8, n8 * 8, true, ov);
+    m[i] = make_float4(fm[0], fm[1], fm[2], fm[3]);
+    v[i] = make_float4(fv[0], fv[1], fv[2], fv[3]);
   }
 }
 
@@ -347,10 +469,11 @@ int mis_adamw8_step(const void* descs, const int* chunk_prefix, int n_tensors, i
   a.max_norm = max_norm;
   a.seed_lo = (uint32_t)seed;
   a.seed_hi = (uint32_t)(seed >> 32);
-  adamw8_step_kernel<<<chunk_end - chunk_begin, A8_THREADS, 0, (hipStream_t)stream>>>(
-      (const Desc8*)descs, chunk_prefix, n_tensors, chunk_begin, a, (const Step8*)step_constants_dev,
-      (const double*)norm_workspace, n_chunks < A8_PARTIALS ? n_chunks : A8_PARTIALS, (uint8_t*)exp_avg,
-      (uint8_t*)exp_avg_scale, (uint8_t*)exp_avg_sq, (uint8_t*)exp_avg_sq_scale, total_norm);
+  const Buffers8 buf{(uint8_t*)exp_avg, (uint8_t*)exp_avg_scale, (uint8_t*)exp_avg_sq, (uint8_t*)exp_avg_sq_scale};
+  const int chunks = chunk_end - chunk_begin, grid = chunks < A8_GRID ? chunks : A8_GRID;
+  adamw8_step_kernel<<<grid, A8_THREADS, 0, (hipStream_t)stream>>>(
+      (const Desc8*)descs, chunk_prefix, n_tensors, chunk_begin, chunks, a, (const Step8*)step_constants_dev,
+      (const double*)norm_workspace, n_chunks < A8_PARTIALS ? n_chunks : A8_PARTIALS, buf, total_norm);
   MIS_CHECK_LAUNCH("adamw8_step");
   return MIS_OK;
 }
@@ -361,12 +484,12 @@ int mis_adamw8_moments(const void* exp_avg, const void* exp_avg_scale, const voi
               "adamw8_moments: bad arguments");
   MIS_REQUIRE((((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq) & 7) == 0 && (((uintptr_t)out_avg | (uintptr_t)out_sq) & 15) == 0,
               "adamw8_moments: misaligned pointer");
-  const int64_t n8 = n_blocks * 16;
-  int64_t grid = (n8 + A8_THREADS - 1) / A8_THREADS;
-  if (grid > 8192) grid = 8192;
+  const int64_t n4 = n_blocks * 32;
+  int64_t grid = (n4 + A8_THREADS - 1) / A8_THREADS;
+  if (grid > 16384) grid = 16384;
   adamw8_moments_kernel<<<(int)grid, A8_THREADS, 0, (hipStream_t)stream>>>(
-      (const uint8_t*)exp_avg, (const uint8_t*)exp_avg_scale, (const uint8_t*)exp_avg_sq, (const uint8_t*)exp_avg_sq_scale, n8,
-      out_avg, out_sq);
+      (const uint32_t*)exp_avg, (const uint8_t*)exp_avg_scale, (const uint32_t*)exp_avg_sq, (const uint8_t*)exp_avg_sq_scale, n4,
+      (float4*)out_avg, (float4*)out_sq);
   MIS_CHECK_LAUNCH("adamw8_moments");
   return MIS_OK;
 }

@@ -440,6 +440,7 @@ class _Table8:
         span = {id(p): s for p, s in zip(plan.params, plan.spans)}
         self.fixed = [(span[id(p)][0] * BLOCK8, p.numel(), F_._DT[p.dtype]) for p in self.order]
         self.plain = [p.is_contiguous() for p in self.order]
+        self.dtypes = [p.dtype for p in self.order]
         self.pointers = self.keep = None
         self.plan_dev = _Plan([f[1] for f in self.fixed], None, prefix, plan.device) if self.order else None
 
@@ -456,10 +457,10 @@ class _Table8:
     def addresses(self):
         """[parameter, gradient, parameter, ...] pointers; a gradient in another memory order than its parameter is copied
         into the parameter's."""
-        dev, out, keep = self.plan.device, [], []
-        for p, plain in zip(self.order, self.plain):
+        dev, out, keep = self.plan.device.index, [], []
+        for p, plain, dtype in zip(self.order, self.plain, self.dtypes):
             g = p.grad
-            if g.dtype is not p.dtype or g.layout is not torch.strided or g.device != dev or p.device != dev:
+            if g.dtype is not dtype or g.is_sparse or g.get_device() != dev or p.get_device() != dev:
                 raise RuntimeError(f"AdamW8 needs dense gradients of the parameter's type and device, got {g.dtype} "
                                    f"{g.layout} on {g.device} for {p.dtype} on {p.device}")
             if not (plain and g.is_contiguous()) and g.stride() != p.stride():
