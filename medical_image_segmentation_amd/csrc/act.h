@@ -11,17 +11,15 @@
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 
-// the two halves of gelu: Phi(u) and e^(-u^2/2)
-__device__ __forceinline__ void gelu_parts(float u, float& phi, float& e) {
-  const float z = fabsf(u);
-  const float t = fast_rcp(fmaf(0.3275911f * 0.70710678f, z, 1.f));
+// the two parts of gelu: q = Phi(-|u|) and e = e^(-u^2/2); the coefficients carry erfc's factor 1/2
+__device__ __forceinline__ void gelu_parts(float u, float& q, float& e) {
+  const float t = fast_rcp(fmaf(0.3275911f * 0.70710678f, fabsf(u), 1.f));
   e = fast_exp2(-0.72134752f * u * u);
-  float p = fmaf(t, 1.061405429f, -1.453152027f);
-  p = fmaf(t, p, 1.421413741f);
-  p = fmaf(t, p, -0.284496736f);
-  p = fmaf(t, p, 0.254829592f);
-  const float q = 0.5f * p * t * e;
-  phi = u >= 0.f ? 1.f - q : q;
+  float p = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+  p = fmaf(t, p, 0.5f * 1.421413741f);
+  p = fmaf(t, p, 0.5f * -0.284496736f);
+  p = fmaf(t, p, 0.5f * 0.254829592f);
+  q = p * (t * e);
 }
 
 template <int ACT>
@@ -31,9 +29,9 @@ __device__ __forceinline__ float act_value(float u) {
   } else if constexpr (ACT == MIS_ACT_SILU) {
     return u * fast_rcp(1.f + fast_exp2(-1.44269504f * u));
   } else if constexpr (ACT == MIS_ACT_GELU) {
-    float phi, e;
-    gelu_parts(u, phi, e);
-    return u * phi;
+    float q, e;                                  // u Phi(u) = max(u, 0) - |u| Phi(-|u|)
+    gelu_parts(u, q, e);
+    return fmaf(-fabsf(u), q, u < 0.f ? 0.f : u);
   } else {
     return u;
   }
@@ -47,9 +45,9 @@ __device__ __forceinline__ float act_slope(float u) {
     const float s = fast_rcp(1.f + fast_exp2(-1.44269504f * u));
     return s * fmaf(u, 1.f - s, 1.f);
   } else if constexpr (ACT == MIS_ACT_GELU) {
-    float phi, e;
-    gelu_parts(u, phi, e);
-    return fmaf(0.39894228f * u, e, phi);
+    float q, e;
+    gelu_parts(u, q, e);
+    return fmaf(0.39894228f * u, e, u < 0.f ? q : 1.f - q);
   } else {
     return 1.f;
   }

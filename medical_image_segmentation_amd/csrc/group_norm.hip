@@ -396,6 +396,27 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_dx_kernel(const T* __restri
 // dy) are read once, the forward is one launch.  Vectors never straddle a group here.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int RES_THREADS = 512, RES_WAVES = RES_THREADS / 64;
+constexpr int RES_WIDE = 256;        // most vectors of a slab side by side
+
+// 64-lane sum of doubles on the DPP path; every lane ends with the total.
+template <int CTRL> __device__ __forceinline__ double dpp_move(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lane_of(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+  v += dpp_move<0xB1>(v);
+  v += dpp_move<0x4E>(v);
+  v += dpp_move<0x141>(v);
+  v += dpp_move<0x140>(v);
+  return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
+}
 
 // Sum over all threads of a group of the two values per thread; valid in red_out[group] after the barrier.
 // Thread tid holds channel vector tid % CV of pixel row tid / CV; a group is GV neighbouring vectors.
@@ -412,11 +433,8 @@ __device__ __forceinline__ void group_sums(double s1, double s2, int CV, int GV,
       t1 += v.x;
       t2 += v.y;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      t1 += __shfl_xor(t1, o, WAVE);
-      t2 += __shfl_xor(t2, o, WAVE);
-    }
+    t1 = wave_sum64(t1);
+    t2 = wave_sum64(t2);
     if (lane == 0) out[g] = make_double2(t1, t2);
   }
   __syncthreads();
@@ -497,8 +515,9 @@ __global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_bwd_kernel(const T
                                                                          const float* __restrict__ gamma,
                                                                          const float* __restrict__ beta, T* __restrict__ dx,
                                                                          float* __restrict__ chan) {
-  __shared__ float2 red[RES_THREADS * V];
-  __shared__ float2 coef[RES_THREADS];
+  __shared__ float red[2 * V * RES_THREADS];             // [channel of the vector][sum][thread]
+  __shared__ float2 tot[RES_WIDE * V];                   // by channel of the slab
+  __shared__ float2 coef[RES_WIDE];
   int b, slab;
   if (!resident_place(s, B, b, slab)) return;
   const Slab sl = slab_of(s, slab);
@@ -517,10 +536,10 @@ __global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_bwd_kernel(const T
   Consts<V> k;
   load_consts<V>(k, stats, gamma, beta, c, s.Cg);
   const float rstd = (float)stats[c / s.Cg].y;
-  if (on) {
-    float a1[V], a2[V];
+  float a1[V], a2[V];
 #pragma unroll
-    for (int j = 0; j < V; j++) a1[j] = a2[j] = 0.f;
+  for (int j = 0; j < V; j++) a1[j] = a2[j] = 0.f;
+  if (on) {
 #pragma unroll
     for (int i = 0; i < NV; i++) {
       if (pr + i * s.PR < HW) {
@@ -533,27 +552,27 @@ __global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_bwd_kernel(const T
         }
       }
     }
+  }
 #pragma unroll
-    for (int j = 0; j < V; j++) red[(pr * s.CV + cv) * V + j] = make_float2(a1[j], a2[j] * rstd);
+  for (int j = 0; j < V; j++) {
+    red[2 * j * RES_THREADS + tid] = a1[j];
+    red[(2 * j + 1) * RES_THREADS + tid] = a2[j] * rstd;
   }
   __syncthreads();
-  const int W = s.CV * V;
-  for (int n = s.PR; n > 1;) {                           // pixel rows: halves onto halves
-    const int h = (n + 1) >> 1;
-    for (int i = tid; i < (n - h) * W; i += RES_THREADS) {
-      if (i % W < sl.nc) {
-        red[i].x += red[i + h * W].x;
-        red[i].y += red[i + h * W].y;
-      }
+  // pixel rows: 16 lanes to a channel and sum
+  float* out = chan + (int64_t)b * 2 * s.C + sl.c0;
+  for (int o = tid >> 4; o < 2 * sl.nc; o += RES_THREADS / 16) {
+    const int ch = o >> 1, which = o & 1, v = ch / V;
+    const float* from = red + (2 * (ch - v * V) + which) * RES_THREADS + v;
+    float t = 0.f;
+    for (int r = tid & 15; r < s.PR; r += 16) t += from[r * s.CV];
+    t = row16_sum(t);
+    if ((tid & 15) == 0) {
+      (which ? tot[ch].y : tot[ch].x) = t;
+      out[which * s.C + ch] = t;
     }
-    __syncthreads();
-    n = h;
   }
-  float* out = chan + (int64_t)b * 2 * s.C;
-  for (int i = tid; i < sl.nc; i += RES_THREADS) {
-    out[sl.c0 + i] = red[i].x;
-    out[s.C + sl.c0 + i] = red[i].y;
-  }
+  __syncthreads();
   if (!dx) return;
   const float inv = (float)(1.0 / ((double)s.HW * s.Cg));
   if (s.Cg <= 16) {                                      // a thread per group, else a wave
@@ -561,8 +580,8 @@ __global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_bwd_kernel(const T
       float t1 = 0.f, t2 = 0.f;
       for (int i = 0; i < s.Cg; i++) {
         const float w = gamma ? gamma[sl.c0 + g * s.Cg + i] : 1.f;
-        t1 = fmaf(w, red[g * s.Cg + i].x, t1);
-        t2 = fmaf(w, red[g * s.Cg + i].y, t2);
+        t1 = fmaf(w, tot[g * s.Cg + i].x, t1);
+        t2 = fmaf(w, tot[g * s.Cg + i].y, t2);
       }
       coef[g] = make_float2(t1 * inv, t2 * inv);
     }
@@ -571,8 +590,8 @@ __global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_bwd_kernel(const T
       float t1 = 0.f, t2 = 0.f;
       for (int i = tid & 63; i < s.Cg; i += 64) {
         const float w = gamma ? gamma[sl.c0 + g * s.Cg + i] : 1.f;
-        t1 = fmaf(w, red[g * s.Cg + i].x, t1);
-        t2 = fmaf(w, red[g * s.Cg + i].y, t2);
+        t1 = fmaf(w, tot[g * s.Cg + i].x, t1);
+        t2 = fmaf(w, tot[g * s.Cg + i].y, t2);
       }
       t1 = wave_sum(t1);
       t2 = wave_sum(t2);
@@ -668,7 +687,7 @@ int plan_resident(Shape& s, int& V, int B, int64_t HW, int C, int G, int esize, 
   const int GV = s.Cg / V;
   auto need = [&](int groups) -> int64_t {              // vectors to a thread
     const int CV = groups * GV;
-    return CV > RES_THREADS ? INT64_MAX : (HW + RES_THREADS / CV - 1) / (RES_THREADS / CV);
+    return CV > RES_WIDE ? INT64_MAX : (HW + RES_THREADS / CV - 1) / (RES_THREADS / CV);
   };
   if (HW > (1 << 20) || need(1) > most) return 0;
   int gps = 1;
@@ -700,6 +719,15 @@ template <typename F> void with_act(int act, F&& f) {
 
 constexpr int RES_FWD = 32, RES_BWD = 16;               // most vectors to a thread
 
+// f(the next power of two from `n` on, at least 2, as a constant)
+template <int MOST, typename F> void with_count(int n, F&& f) {
+  if (n <= 2) f(std::integral_constant<int, 2>());
+  else if (n <= 4) f(std::integral_constant<int, 4>());
+  else if (n <= 8) f(std::integral_constant<int, 8>());
+  else if (n <= 16) f(std::integral_constant<int, 16>());
+  else f(std::integral_constant<int, MOST>());
+}
+
 int resident_grid(const Shape& s, int B) { return (B * s.slabs + 7) / 8 * 8; }
 
 template <typename T, int V>
@@ -708,9 +736,9 @@ void launch_resident_fwd(const T* x, const Shape& s, int nv, int B, const float*
   const int grid = resident_grid(s, B);
   with_act(act, [&](auto a) {
     constexpr int ACT = decltype(a)::value;
-    if (nv <= 2) gn_resident_kernel<T, V, 2, ACT><<<grid, RES_THREADS, 0, st>>>(x, s, B, eps, gamma, beta, y, stats);
-    else if (nv <= 8) gn_resident_kernel<T, V, 8, ACT><<<grid, RES_THREADS, 0, st>>>(x, s, B, eps, gamma, beta, y, stats);
-    else gn_resident_kernel<T, V, RES_FWD, ACT><<<grid, RES_THREADS, 0, st>>>(x, s, B, eps, gamma, beta, y, stats);
+    with_count<RES_FWD>(nv, [&](auto n) {
+      gn_resident_kernel<T, V, decltype(n)::value, ACT><<<grid, RES_THREADS, 0, st>>>(x, s, B, eps, gamma, beta, y, stats);
+    });
   });
 }
 
@@ -720,12 +748,9 @@ void launch_resident_bwd(const T* x, const T* dy, const Shape& s, int nv, int B,
   const int grid = resident_grid(s, B);
   with_act(act, [&](auto a) {
     constexpr int ACT = decltype(a)::value;
-    if (nv <= 2)
-      gn_resident_bwd_kernel<T, V, 2, ACT><<<grid, RES_THREADS, 0, st>>>(x, dy, s, B, stats, gamma, beta, dx, chan);
-    else if (nv <= 8)
-      gn_resident_bwd_kernel<T, V, 8, ACT><<<grid, RES_THREADS, 0, st>>>(x, dy, s, B, stats, gamma, beta, dx, chan);
-    else
-      gn_resident_bwd_kernel<T, V, RES_BWD, ACT><<<grid, RES_THREADS, 0, st>>>(x, dy, s, B, stats, gamma, beta, dx, chan);
+    with_count<RES_BWD>(nv, [&](auto n) {
+      gn_resident_bwd_kernel<T, V, decltype(n)::value, ACT><<<grid, RES_THREADS, 0, st>>>(x, dy, s, B, stats, gamma, beta, dx, chan);
+    });
   });
   if (dgamma || dbeta)
     gn_bwd_finish_kernel<<<cdiv(s.C, 64), 256, 0, st>>>(chan, gamma, B, s.C, s.Cg, s.G, 1.0, cdiv(s.C, 64), nullptr, dgamma, dbeta);

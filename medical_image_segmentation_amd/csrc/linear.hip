@@ -566,20 +566,57 @@ __global__ __launch_bounds__(256) void lin_pad_kernel(const T* __restrict__ src,
   }
 }
 
-// rows[chunk][N] = sums of a chunk's rows of d (row stride ld)
-constexpr int SUM_ROWS = 256;
-template <typename T>
-__global__ __launch_bounds__(256) void lin_colsum_kernel(const T* __restrict__ d, int64_t ld, int64_t M, int N,
-                                                         float* __restrict__ rows) {
-  __shared__ float red[4][64];
-  const int c = blockIdx.y * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
-  const int64_t m1 = min((int64_t)(blockIdx.x + 1) * SUM_ROWS, M);
-  float s = 0.f;
-  if (c < N)
-    for (int64_t m = (int64_t)blockIdx.x * SUM_ROWS + w; m < m1; m += 4) s += to_f32(d[m * ld + c]);
-  red[w][threadIdx.x & 63] = s;
+// rows[chunk][N] = sums of a chunk's rows of d (row stride ld); a thread has V neighbouring columns, up to 64 threads side
+// by side, the others take rows in turn.  Chunks of 256 rows, shorter down to 32 while there are fewer than 1024 blocks.
+int sum_rows(int64_t M, int64_t N) {
+  int rows = 256;
+  while (rows > 32 && (int64_t)cdiv(M, rows) * cdiv(N, 512) < 1024) rows /= 2;
+  return rows;
+}
+template <typename T, int V>
+__global__ __launch_bounds__(256) void lin_colsum_kernel(const T* __restrict__ d, int64_t ld, int64_t M, int N, int side,
+                                                         int chunk, float* __restrict__ rows) {
+  __shared__ float red[256 * V];
+  const int cx = threadIdx.x % side, w = threadIdx.x / side, lanes = 256 / side;
+  const int c = (blockIdx.y * side + cx) * V;
+  const int64_t m1 = min((int64_t)(blockIdx.x + 1) * chunk, M);
+  float s[V];
+#pragma unroll
+  for (int k = 0; k < V; k++) s[k] = 0.f;
+  if (c < N && w < lanes) {
+#pragma unroll 8
+    for (int64_t m = (int64_t)blockIdx.x * chunk + w; m < m1; m += lanes) {
+      if constexpr (V == 1) {
+        s[0] += to_f32(d[m * ld + c]);
+      } else {
+        Pack<T> x;
+        x.load(d + m * ld + c);
+#pragma unroll
+        for (int k = 0; k < V; k++) s[k] += x.v[k];
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < V; k++) red[k * 256 + threadIdx.x] = s[k];
   __syncthreads();
-  if (w == 0 && c < N) rows[(int64_t)blockIdx.x * N + c] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+  for (int i = threadIdx.x; i < side * V; i += 256) {
+    const int x = i / V, k = i - x * V, col = (blockIdx.y * side + x) * V + k;
+    float t = 0.f;
+    for (int l = 0; l < lanes; l++) t += red[k * 256 + l * side + x];
+    if (col < N) rows[(int64_t)blockIdx.x * N + col] = t;
+  }
+}
+
+template <typename T>
+void launch_colsum(const T* d, int64_t ld, int64_t M, int64_t N, float* rows, float* out, hipStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const bool wide = ((uintptr_t)d & 15) == 0 && ld % V == 0 && N % V == 0;
+  const int per = wide ? V : 1, side = (int)(N / per < 64 ? (N + per - 1) / per : 64);
+  const int chunk = sum_rows(M, N);
+  const dim3 grid(cdiv(M, chunk), cdiv(N, (int64_t)side * per));
+  if (wide) lin_colsum_kernel<T, V><<<grid, 256, 0, st>>>(d, ld, M, (int)N, side, chunk, rows);
+  else lin_colsum_kernel<T, 1><<<grid, 256, 0, st>>>(d, ld, M, (int)N, side, chunk, rows);
+  launch_reduce_partials(rows, cdiv(M, chunk), (int)N, out, st);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -738,7 +775,7 @@ template <typename T> struct Buffers {
     w = s.take<T>(Kp != K ? N * Kp : 0);
     z = s.take<T>(!backward ? 0 : act != MIS_ACT_NONE || Np != N ? M * Np : 0);       // dz, or a padded dy
     size_t most = part_floats(sizeof(T), N, M, K), few_rows = most ? JOIN_Q : 64;
-    rows = s.take<float>(!backward ? 0 : act == MIS_ACT_NONE ? (size_t)cdiv(M, SUM_ROWS) * N : (M + few_rows - 1) / few_rows * N);
+    rows = s.take<float>(!backward ? 0 : act == MIS_ACT_NONE ? (size_t)cdiv(M, sum_rows(M, N)) * N : (M + few_rows - 1) / few_rows * N);
     if (backward)
       for (size_t n : {part_floats(sizeof(T), K, M, N), part_floats(sizeof(T), K, N, M)})
         if (n > most) most = n;
@@ -816,8 +853,7 @@ int backward(const T* x, int64_t ldx, const T* w, const float* bias, const T* dy
     ldz = Np;
     if (db) launch_reduce_partials(buf.rows, cdiv(M, cut.row_tiles()), (int)N, db, st);
   } else if (db) {
-    lin_colsum_kernel<T><<<dim3(cdiv(M, SUM_ROWS), cdiv(N, 64)), 256, 0, st>>>(dy, ldd, M, (int)N, buf.rows);
-    launch_reduce_partials(buf.rows, cdiv(M, SUM_ROWS), (int)N, db, st);
+    launch_colsum(dy, ldd, M, N, buf.rows, db, st);
   }
   if (staged && pad_dy && (dx || dw)) {
     z = pad(dy, M, N, ldd, buf.z, st);
