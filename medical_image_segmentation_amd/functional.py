@@ -9,7 +9,6 @@ stored channels-last (`memory_format=torch.channels_last`), dtype float32 or
 bfloat16.  Parameters are float32 in the reference's own layouts.
 """
 import ctypes
-import functools
 import os
 import weakref
 
@@ -1866,26 +1865,21 @@ class _on_device_of:
         return False
 
 
-_scratch_bytes = functools.lru_cache(maxsize=4096)(query)      # (name, sizes) -> bytes: a pure function of the sizes
+_NATIVE = None
 
 
-def _enqueue(name, x, nbytes, prof, *args):
-    """call(name, *args, scratch of `nbytes`, stream) on the current stream of x's device.  prof = (family, flops, bytes).
-    While a HIP graph is being captured the scratch comes from that graph's own pool, so that two captured graphs never
-    share a buffer; else it is `workspace`.  (Small calls are bound by the host: no context managers on the usual way.)"""
-    idx = x.get_device()
-    if idx != torch.cuda.current_device():
-        with torch.cuda.device(idx):
-            return _enqueue(name, x, nbytes, prof, *args)
-    if torch.cuda.is_current_stream_capturing():
-        ws = torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=x.device)
-    else:
-        ws = workspace(nbytes, x.device)
-    if PROFILE is None:
-        call(name, *args, ws.data_ptr(), _stream())
-    else:
-        with _prof(*prof):
-            call(name, *args, ws.data_ptr(), _stream())
+def _native():
+    """The C++ autograd nodes of the operators below (csrc/torch_ops.cpp, built with the library)."""
+    global _NATIVE
+    if _NATIVE is None:
+        _lib.load()
+        try:
+            from . import _ops
+        except ImportError as e:
+            raise RuntimeError(f"the autograd extension _ops.so cannot be loaded ({e}): build it with `make -C "
+                               f"{os.path.join(os.path.dirname(_lib.LIB_PATH), 'csrc')}`") from e
+        _NATIVE = _ops
+    return _NATIVE
 
 
 def _check_param(t, n, name, like):
@@ -1895,45 +1889,6 @@ def _check_param(t, n, name, like):
         raise ValueError(f"{name}: expected float32 [{n}], got {t.dtype} {tuple(t.shape)}")
     if t.device != like.device:
         raise RuntimeError(f"{name} is on {t.device}, the input on {like.device}")
-
-
-class GroupNormActFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, act):
-        B, Cc, H, W = x.shape
-        weight = weight.contiguous() if weight is not None else None
-        bias = bias.contiguous() if bias is not None else None
-        y = torch.empty_like(x, memory_format=torch.channels_last)
-        stats = torch.empty((B, groups, 2), dtype=torch.float64, device=x.device)
-        n, dt = x.numel(), _DT[x.dtype]
-        if n:
-            _enqueue("mis_group_norm_act_fwd", x,
-                     _scratch_bytes("mis_group_norm_act_fwd_workspace_bytes", dt, B, H * W, Cc, groups),
-                     ("group_norm_act_fwd", 8 * n, 2 * n * x.element_size()),
-                     x.data_ptr(), dt, B, H * W, Cc, groups, _p(weight), _p(bias), eps, act, y.data_ptr(), stats.data_ptr())
-        ctx.save_for_backward(x, weight, bias, stats)
-        ctx.groups, ctx.act = groups, act
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, stats = ctx.saved_tensors
-        B, Cc, H, W = x.shape
-        n, dt = x.numel(), _DT[x.dtype]
-        if n and not (dy.dtype == x.dtype and dy.is_contiguous(memory_format=torch.channels_last)):
-            dy = to_act(dy, x.dtype)
-        dx = torch.empty_like(x, memory_format=torch.channels_last) if ctx.needs_input_grad[0] else None
-        grad = torch.empty if n else torch.zeros
-        dw = grad(Cc, dtype=torch.float32, device=x.device) if ctx.needs_input_grad[1] else None
-        db = grad(Cc, dtype=torch.float32, device=x.device) if ctx.needs_input_grad[2] else None
-        if n:
-            _enqueue("mis_group_norm_act_bwd", x,
-                     _scratch_bytes("mis_group_norm_act_bwd_workspace_bytes", dt, B, H * W, Cc, ctx.groups),
-                     ("group_norm_act_bwd", 22 * n, 3 * n * x.element_size()),
-                     x.data_ptr(), dy.data_ptr(), dt, B, H * W, Cc, ctx.groups, _p(weight), _p(bias), stats.data_ptr(),
-                     ctx.act, _p(dx), _p(dw), _p(db))
-        return dx, dw, db, None, None, None
 
 
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="none"):
@@ -1948,61 +1903,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="
         raise ValueError(f"eps must not be negative, got {eps}")
     _check_param(weight, x.shape[1], "weight", x)
     _check_param(bias, x.shape[1], "bias", x)
-    return GroupNormActFn.apply(x, weight, bias, num_groups, float(eps), act)
-
-
-def _as_rows(t, n):
-    """[..., n] -> ([rows, n] with contiguous rows, row stride); a copy only where the strides need one."""
-    if t.is_contiguous():
-        return t, n
-    t = t.reshape(-1, n)
-    if t.stride(1) != 1 and n > 1 or t.shape[0] > 1 and t.stride(0) < n:
-        t = t.contiguous()
-    return t, (t.stride(0) if t.shape[0] > 1 else n)
-
-
-class LinearActFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, act):
-        N, K = weight.shape
-        w = weight.contiguous()
-        bias = bias.contiguous() if bias is not None else None
-        x2, ldx = _as_rows(x, K)
-        r2, ldr = _as_rows(residual, N) if residual is not None else (None, 0)
-        M, dt = x.numel() // K, _DT[x.dtype]
-        y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
-        if M:
-            nbytes = (M * K + N * K + M * N * (1 if r2 is None else 2)) * x.element_size()
-            _enqueue("mis_linear_act_fwd", x, _scratch_bytes("mis_linear_act_fwd_workspace_bytes", dt, M, N, K),
-                     ("linear_act_fwd", 2 * M * N * K, nbytes),
-                     x2.data_ptr(), ldx, w.data_ptr(), _p(bias), _p(r2), ldr, dt, M, N, K, act, y.data_ptr())
-        ctx.save_for_backward(x, w, bias)
-        ctx.act = act
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, w, bias = ctx.saved_tensors
-        N, K = w.shape
-        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
-        dr = dy if need_r else None
-        if not (need_x or need_w or need_b):
-            return None, None, None, dr, None
-        x2, ldx = _as_rows(x, K)
-        d2, ldd = _as_rows(dy if dy.dtype == x.dtype else dy.to(x.dtype), N)
-        M, dt = x.numel() // K, _DT[x.dtype]
-        grad = torch.empty if M else torch.zeros
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        dw = grad((N, K), dtype=x.dtype, device=x.device) if need_w else None
-        db = grad(N, dtype=torch.float32, device=x.device) if need_b else None
-        if M:
-            nbytes = (2 * M * K + 2 * N * K + M * N) * x.element_size()
-            _enqueue("mis_linear_act_bwd", x, _scratch_bytes("mis_linear_act_bwd_workspace_bytes", dt, M, N, K, ctx.act),
-                     ("linear_act_bwd", 4 * M * N * K, nbytes),
-                     x2.data_ptr(), ldx, w.data_ptr(), _p(bias), d2.data_ptr(), ldd, dt, M, N, K, ctx.act, _p(dx), _p(dw),
-                     _p(db))
-        return dx, dw, db, dr, None
+    return _native().group_norm_act(x, weight, bias, num_groups, float(eps), act)
 
 
 def linear_act(x, weight, bias=None, activation="none", residual=None):
@@ -2026,7 +1927,7 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
     if residual is not None and residual.shape != x.shape[:-1] + (weight.shape[0],):
         raise ValueError(f"residual {tuple(residual.shape)}: expected {tuple(x.shape[:-1]) + (weight.shape[0],)}")
     _check_param(bias, weight.shape[0], "bias", x)
-    return LinearActFn.apply(x, weight, bias, residual, act)
+    return _native().linear_act(x, weight, bias, residual, act)
 
 
 def pointwise_conv_act(x, weight, bias=None, activation="none", residual=None):

@@ -457,7 +457,10 @@ class _Table8:
     def addresses(self):
         """[parameter, gradient, parameter, ...] pointers; a gradient in another memory order than its parameter is copied
         into the parameter's."""
-        dev, out, keep = self.plan.device.index, [], []
+        dev, keep = self.plan.device.index, []
+        out = F_._native().step_pointers(self.order, dev)
+        if out:
+            return out, keep
         for p, plain, dtype in zip(self.order, self.plain, self.dtypes):
             g = p.grad
             if g.dtype is not dtype or g.is_sparse or g.get_device() != dev or p.get_device() != dev:

@@ -429,6 +429,30 @@ def test_results_repeat_bit_for_bit():
         assert all(torch.equal(s, t) for s, t in zip(a, _both(F_, x, w, b, wl)))
 
 
+def test_a_second_derivative_is_refused():
+    """The backward is not differentiable: asking for its derivative raises, asking for a graph alone does not."""
+    from medical_image_segmentation_amd import functional as F_
+    x = _x((1, 8, 4, 4), torch.float32, 80).requires_grad_(True)
+    w = torch.randn((8, 8), device=DEV, requires_grad=True)
+    for y in (F_.group_norm_act(x, 2, activation="silu"), F_.pointwise_conv_act(x, w, None, "gelu")):
+        g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        assert g.requires_grad
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(g.sum(), x)
+
+
+def test_backward_accumulates_into_leaves():
+    from medical_image_segmentation_amd import functional as F_
+    x, w = torch.randn((6, 16), device=DEV, requires_grad=True), torch.randn((8, 16), device=DEV, requires_grad=True)
+    r = torch.randn((6, 8), device=DEV, requires_grad=True)
+    dy = torch.randn((6, 8), device=DEV)
+    want = torch.autograd.grad(F_.linear_act(x, w, None, "silu", r), [x, w, r], dy)
+    for _ in range(2):
+        F_.linear_act(x, w, None, "silu", r).backward(dy)
+    for t, g in zip((x, w, r), want):
+        assert torch.equal(t.grad, g + g)
+
+
 def test_channel_mlp_trains_with_adamw8():
     """Norm, widening product, narrowing product with the skip, and the optimizer together: outputs and gradients of the
     block against 64 bits, then three optimizer steps that stay finite and move every parameter."""
