@@ -135,6 +135,33 @@ __global__ __launch_bounds__(GN_THREADS) void gn_sums_kernel(const T* __restrict
   }
 }
 
+// 64-lane sum of doubles on the DPP path; every lane ends with the total.
+template <int CTRL> __device__ __forceinline__ double dpp_move(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lane_of(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+  v += dpp_move<0xB1>(v);
+  v += dpp_move<0x4E>(v);
+  v += dpp_move<0x141>(v);
+  v += dpp_move<0x140>(v);
+  return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
+}
+
+__device__ __forceinline__ double2 stats_of(double s1, double s2, double count, double eps) {
+  const double mean = s1 / count;
+  double var = s2 / count - mean * mean;
+  if (var < 0.0) var = 0.0;                              // (NaN stays NaN)
+  return make_double2(mean, 1.0 / sqrt(var + eps));
+}
+
 // stats[b][g] = (mean, 1/sqrt(var + eps)); one wave per (b, g)
 __global__ __launch_bounds__(64) void gn_stats_kernel(const double2* __restrict__ sums, int rows, int G, double count,
                                                       double eps, double2* __restrict__ stats) {
@@ -145,17 +172,9 @@ __global__ __launch_bounds__(64) void gn_stats_kernel(const double2* __restrict_
     t1 += v.x;
     t2 += v.y;
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    t1 += __shfl_xor(t1, o, WAVE);
-    t2 += __shfl_xor(t2, o, WAVE);
-  }
-  if (lane == 0) {
-    const double mean = t1 / count;
-    double var = t2 / count - mean * mean;
-    if (var < 0.0) var = 0.0;                            // (NaN stays NaN)
-    stats[(int64_t)b * G + g] = make_double2(mean, 1.0 / sqrt(var + eps));
-  }
+  t1 = wave_sum64(t1);
+  t2 = wave_sum64(t2);
+  if (lane == 0) stats[(int64_t)b * G + g] = stats_of(t1, t2, count, eps);
 }
 
 // What a thread holds of its V channels: u = (x - mean) * a + beta, a = rstd * gamma.
@@ -163,29 +182,75 @@ template <int V> struct Consts {
   float mean[V], a[V], beta[V];
 };
 
-template <int V>
-__device__ __forceinline__ void load_consts(Consts<V>& k, const double2* __restrict__ stats, const float* __restrict__ gamma,
-                                            const float* __restrict__ beta, int c, int Cg) {
+// f(i, group of channel c + i, whether that is another group than channel c + i - 1's) for i < V, with one division.
+template <int V, typename F> __device__ __forceinline__ void with_groups(int c, int Cg, F&& f) {
+  int g = c / Cg, left = Cg - (c - g * Cg);
 #pragma unroll
   for (int i = 0; i < V; i++) {
-    const double2 st = stats[(c + i) / Cg];
-    k.mean[i] = (float)st.x;
-    k.a[i] = (float)st.y * (gamma ? gamma[c + i] : 1.f);
-    k.beta[i] = beta ? beta[c + i] : 0.f;
+    const bool other = i > 0 && left == 0;
+    if (other) {
+      g++;
+      left = Cg;
+    }
+    f(i, g, i == 0 || other);
+    left--;
   }
 }
 
-template <typename T, int V, int ACT>
-__global__ __launch_bounds__(GN_THREADS) void gn_apply_kernel(const T* __restrict__ x, Shape s, const double2* __restrict__ stats,
+template <int V>
+__device__ __forceinline__ void load_consts(Consts<V>& k, const double2* __restrict__ stats, const float* __restrict__ gamma,
+                                            const float* __restrict__ beta, int c, int Cg) {
+  double2 st = make_double2(0.0, 0.0);
+  with_groups<V>(c, Cg, [&](int i, int g, bool other) {
+    if (other) st = stats[g];
+    k.mean[i] = (float)st.x;
+    k.a[i] = (float)st.y;
+  });
+#pragma unroll
+  for (int i = 0; i < V; i++) k.beta[i] = beta ? beta[c + i] : 0.f;
+  if (gamma) {
+#pragma unroll
+    for (int i = 0; i < V; i++) k.a[i] *= gamma[c + i];
+  }
+}
+
+// FOLD: the workgroup adds up the rows of `sums` of its own few groups itself (a launch less on the way to y) and the one
+// of the first chunk leaves the statistics.  Up to 64 rows: 2x32x128^2 bf16 12.1 -> 9.9 us; at the 128 rows of the large
+// tensors every workgroup's start gets longer by more than the launch cost (16x32x512^2 171 -> 178 us).
+constexpr int FOLD_GROUPS = 16, FOLD_ROWS = 64;
+template <typename T, int V, int ACT, bool FOLD>
+__global__ __launch_bounds__(GN_THREADS) void gn_apply_kernel(const T* __restrict__ x, Shape s, const double2* __restrict__ sums,
+                                                              double eps, double2* __restrict__ stats_all,
                                                               const float* __restrict__ gamma, const float* __restrict__ beta,
                                                               T* __restrict__ y) {
+  __shared__ double2 own[FOLD_GROUPS];
   const int b = blockIdx.z, tid = threadIdx.x;
   const Slab sl = slab_of(s, blockIdx.y);
   const int cv = tid % s.CV, pr = tid / s.CV;
+  double2* stats = stats_all + (int64_t)b * s.G;
+  if constexpr (FOLD) {
+    const int lane = tid & 63, rows = s.chunks * s.parts;
+    const double count = (double)s.HW * s.Cg;
+    for (int g = tid >> 6; g < sl.ng; g += GN_THREADS / 64) {
+      double t1 = 0.0, t2 = 0.0;
+#pragma unroll 4
+      for (int r = lane; r < rows; r += 64) {
+        const double2 v = sums[((int64_t)b * rows + r) * s.G + sl.g0 + g];
+        t1 += v.x;
+        t2 += v.y;
+      }
+      const double2 st = stats_of(wave_sum64(t1), wave_sum64(t2), count, eps);
+      if (lane == 0) {
+        own[g] = st;
+        if (blockIdx.x == 0) stats[sl.g0 + g] = st;      // (the parts of one group write the same)
+      }
+    }
+    __syncthreads();
+  }
   if (pr >= s.PR || cv * V >= sl.nc) return;
   const int c = sl.c0 + cv * V;
   Consts<V> k;
-  load_consts<V>(k, stats + (int64_t)b * s.G, gamma, beta, c, s.Cg);
+  load_consts<V>(k, FOLD ? own - sl.g0 : stats, gamma, beta, c, s.Cg);
   const int64_t p0 = (int64_t)blockIdx.x * s.ppc, p1 = min(p0 + s.ppc, s.HW);
   const int64_t base = (int64_t)b * s.HW * s.C + c;
 #pragma unroll 4
@@ -252,9 +317,11 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_sums_kernel(const T* __rest
         a2[i] = fmaf(du, xf - k.mean[i], a2[i]);         // times rstd at the end
       }
     }
-#pragma unroll
-    for (int i = 0; i < V; i++)
-      red[(pr * s.CV + cv) * V + i] = make_float2(a1[i], a2[i] * (float)stats[(c + i) / s.Cg].y);
+    float rstd = 0.f;
+    with_groups<V>(c, s.Cg, [&](int i, int g, bool other) {
+      if (other) rstd = (float)stats[g].y;
+      red[(pr * s.CV + cv) * V + i] = make_float2(a1[i], a2[i] * rstd);
+    });
   }
   __syncthreads();
   const int W = s.CV * V;
@@ -278,16 +345,17 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_sums_kernel(const T* __rest
   }
 }
 
-// chan[b][2][C] = sums over the chunks; block = 32 channels of one sample, 8 row lanes
-__global__ __launch_bounds__(256) void gn_bwd_channels_kernel(const float* __restrict__ rows, int chunks, int C,
-                                                              float* __restrict__ chan) {
-  __shared__ double2 red[8][33];
+// chan[b][2][C] = sums over the chunks; block = 32 channels of one sample, R row lanes
+template <int R>
+__global__ __launch_bounds__(32 * R) void gn_bwd_channels_kernel(const float* __restrict__ rows, int chunks, int C,
+                                                                 float* __restrict__ chan) {
+  __shared__ double2 red[R][33];
   const int lane = threadIdx.x & 31, r = threadIdx.x >> 5, c = blockIdx.x * 32 + lane, b = blockIdx.y;
   double t1 = 0.0, t2 = 0.0;
   if (c < C) {
     const float* p = rows + (int64_t)b * chunks * 2 * C + c;
-#pragma unroll 4
-    for (int i = r; i < chunks; i += 8) {
+#pragma unroll 8
+    for (int i = r; i < chunks; i += R) {
       t1 += (double)p[(int64_t)i * 2 * C];
       t2 += (double)p[(int64_t)i * 2 * C + C];
     }
@@ -295,7 +363,8 @@ __global__ __launch_bounds__(256) void gn_bwd_channels_kernel(const float* __res
   red[r][lane] = make_double2(t1, t2);
   __syncthreads();
   if (r == 0 && c < C) {
-    for (int i = 1; i < 8; i++) {
+#pragma unroll
+    for (int i = 1; i < R; i++) {
       t1 += red[i][lane].x;
       t2 += red[i][lane].y;
     }
@@ -366,14 +435,16 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_dx_kernel(const T* __restri
   Consts<V> k;
   load_consts<V>(k, stats, gamma, beta, c, s.Cg);
   float q1[V], q2[V];                                    // dx = du a - q1 - (x - mean) q2
-#pragma unroll
-  for (int i = 0; i < V; i++) {
-    const int g = (c + i) / s.Cg;
-    const float rstd = (float)stats[g].y;
-    const float2 m = coef[(int64_t)b * s.G + g];
+  float rstd = 0.f;
+  float2 m = make_float2(0.f, 0.f);
+  with_groups<V>(c, s.Cg, [&](int i, int g, bool other) {
+    if (other) {
+      rstd = (float)stats[g].y;
+      m = coef[(int64_t)b * s.G + g];
+    }
     q1[i] = rstd * m.x;
     q2[i] = rstd * rstd * m.y;
-  }
+  });
   const int64_t p0 = (int64_t)blockIdx.x * s.ppc, p1 = min(p0 + s.ppc, s.HW);
   const int64_t base = (int64_t)b * s.HW * s.C + c;
 #pragma unroll 2
@@ -397,26 +468,6 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_dx_kernel(const T* __restri
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int RES_THREADS = 512, RES_WAVES = RES_THREADS / 64;
 constexpr int RES_WIDE = 256;        // most vectors of a slab side by side
-
-// 64-lane sum of doubles on the DPP path; every lane ends with the total.
-template <int CTRL> __device__ __forceinline__ double dpp_move(double v) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, true);
-  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, true);
-  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-__device__ __forceinline__ double lane_of(double v, int lane) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
-  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-__device__ __forceinline__ double wave_sum64(double v) {
-  v += dpp_move<0xB1>(v);
-  v += dpp_move<0x4E>(v);
-  v += dpp_move<0x141>(v);
-  v += dpp_move<0x140>(v);
-  return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
-}
 
 // Sum over all threads of a group of the two values per thread; valid in red_out[group] after the barrier.
 // Thread tid holds channel vector tid % CV of pixel row tid / CV; a group is GV neighbouring vectors.
@@ -485,10 +536,7 @@ __global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_kernel(const T* __
   group_sums(s1, s2, s.CV, GV, sl.ng, s.PR, red, grp);
   const double count = (double)s.HW * s.Cg;
   if (tid < sl.ng) {
-    const double mean = grp[tid].x / count;
-    double var = grp[tid].y / count - mean * mean;
-    if (var < 0.0) var = 0.0;                            // (NaN stays NaN)
-    const double2 st = make_double2(mean, 1.0 / sqrt(var + eps));
+    const double2 st = stats_of(grp[tid].x, grp[tid].y, count, eps);
     grp[tid] = st;
     stats[(int64_t)b * s.G + sl.g0 + tid] = st;
   }
@@ -767,9 +815,12 @@ void launch_fwd(const T* x, const Shape& s, int B, const float* gamma, const flo
   if (s.Cg % V == 0) sum(std::integral_constant<int, V>());
   else if (V >= 4 && s.Cg % (V / 2) == 0) sum(std::integral_constant<int, (V >= 4 ? V / 2 : 1)>());
   else sum(std::integral_constant<int, 1>());
-  gn_stats_kernel<<<dim3(s.G, B), 64, 0, st>>>(sums, s.chunks * s.parts, s.G, (double)s.HW * s.Cg, eps, stats);
+  const bool fold = (s.parts == 1 ? s.gps : 1) <= FOLD_GROUPS && s.chunks * s.parts <= FOLD_ROWS;
+  if (!fold) gn_stats_kernel<<<dim3(s.G, B), 64, 0, st>>>(sums, s.chunks * s.parts, s.G, (double)s.HW * s.Cg, eps, stats);
   with_act(act, [&](auto a) {
-    gn_apply_kernel<T, V, decltype(a)::value><<<grid, GN_THREADS, 0, st>>>(x, s, stats, gamma, beta, y);
+    constexpr int ACT = decltype(a)::value;
+    if (fold) gn_apply_kernel<T, V, ACT, true><<<grid, GN_THREADS, 0, st>>>(x, s, sums, eps, stats, gamma, beta, y);
+    else gn_apply_kernel<T, V, ACT, false><<<grid, GN_THREADS, 0, st>>>(x, s, sums, eps, stats, gamma, beta, y);
   });
 }
 
@@ -784,13 +835,13 @@ void launch_bwd_act(const T* x, const T* dy, const Shape& s, int B, const float*
   const dim3 grid(s.chunks, s.slabs, B);
   const size_t lds = (size_t)s.PR * s.CV * V * sizeof(float2);
   gn_bwd_sums_kernel<T, V, ACT><<<grid, GN_THREADS, lds, st>>>(x, dy, s, stats, gamma, beta, w.rows);
-  gn_bwd_channels_kernel<<<dim3(cdiv(s.C, 32), B), 256, 0, st>>>(w.rows, s.chunks, s.C, w.chan);
+  if (s.chunks > 64) gn_bwd_channels_kernel<32><<<dim3(cdiv(s.C, 32), B), 1024, 0, st>>>(w.rows, s.chunks, s.C, w.chan);
+  else gn_bwd_channels_kernel<8><<<dim3(cdiv(s.C, 32), B), 256, 0, st>>>(w.rows, s.chunks, s.C, w.chan);
   const int channel_blocks = dgamma || dbeta ? cdiv(s.C, 64) : 0, coef_blocks = dx ? cdiv((int64_t)B * s.G, 4) : 0;
   if (channel_blocks + coef_blocks > 0)
     gn_bwd_finish_kernel<<<channel_blocks + coef_blocks, 256, 0, st>>>(w.chan, gamma, B, s.C, s.Cg, s.G, (double)s.HW * s.Cg,
                                                                       channel_blocks, w.coef, dgamma, dbeta);
-  if (!dx) return;
-  gn_bwd_dx_kernel<T, V, ACT><<<grid, GN_THREADS, 0, st>>>(x, dy, s, stats, gamma, beta, w.coef, dx);
+  if (dx) gn_bwd_dx_kernel<T, V, ACT><<<grid, GN_THREADS, 0, st>>>(x, dy, s, stats, gamma, beta, w.coef, dx);
 }
 
 template <typename T, int V>
