@@ -637,11 +637,11 @@ struct Cut {
 // The cheapest by a model of the time in microseconds: rounds of workgroups over the chip's 256 CUs; a round = start,
 // epilogue and its stages, a stage at the matrix rate of the tile (shared by the workgroups of a CU) or, for a lone
 // workgroup, at the time a load takes; for a split sum the second launch, and the parts written and read.  The constants
-// are fitted to 78 products of 1 to 10^6 rows and 24 to 4096 columns, forward and both backward ones, bf16 and float32,
-// each measured in all cuts: the choice is 2 % slower than the best cut on average, 30 % at worst (a 20 us product).
+// are fitted to 160 products of 1 to 10^6 rows and 24 to 4096 columns, forward and the three backward ones, bf16 and
+// float32, each measured in all cuts: the choice is 2 % slower than the best cut on average, 29 % at worst (14 us for 11).
 Cut pick_cut(int esize, bool staged, int64_t p, int64_t q, int64_t r) {
-  struct Rate { double full, alone; int at_a_time; };
-  static const Rate rates[] = {{0.8, 1.2, 3}, {0.185, 0.46, 3}, {0.50, 0.90, 2}, {2.0, 0.90, 1}};      // by Tile
+  struct Rate { double full, alone, per_output; int at_a_time; };
+  static const Rate rates[] = {{0.8, 1.2, 3e-5, 3}, {0.057, 0.45, 3e-5, 3}, {0.41, 0.745, 3e-5, 2}, {1.06, 0.2, 7e-5, 1}};   // by Tile
   const int K = ROW_BYTES / esize;
   const int64_t stages = (r + K - 1) / K;
   Cut best{ANY64, 1, stages * K, 1e300};
@@ -649,8 +649,8 @@ Cut pick_cut(int esize, bool staged, int64_t p, int64_t q, int64_t r) {
     const int edge = tile_edge((Tile)t), slots = 256 * rates[t].at_a_time;
     const int64_t tiles = (int64_t)cdiv(p, edge) * cdiv(q, edge);
     auto round_us = [&](int64_t wgs, int64_t per) {
-      const double share = wgs > 256 ? wgs / 256.0 : 1.0, full = rates[t].full * (esize == 4 ? 2.8 : 1.0) * share;
-      return 2.9 + 3e-5 * edge * edge * share + per * (full > rates[t].alone ? full : rates[t].alone);
+      const double share = wgs > 256 ? wgs / 256.0 : 1.0, full = rates[t].full * (esize == 4 ? 1.84 : 1.0) * share;
+      return 2.6 + rates[t].per_output * edge * edge * share + per * (full > rates[t].alone ? full : rates[t].alone);
     };
     for (int s = 1; s <= 1024; s *= 2) {
       const int64_t per = (stages + s - 1) / s;
@@ -658,7 +658,7 @@ Cut pick_cut(int esize, bool staged, int64_t p, int64_t q, int64_t r) {
       if (s > 1 && (splits == 1 || per < 2 || tiles * splits > 4096)) break;
       const int64_t wgs = tiles * splits, rounds = (wgs + slots - 1) / slots;
       double us = (rounds - 1) * round_us(slots, per) + round_us(wgs - (rounds - 1) * slots, per);
-      if (splits > 1) us += 2.9 + 3.1e-6 * splits * p * q;
+      if (splits > 1) us += 2.6 + 3.1e-6 * splits * p * q;
       if (us < best.us) best = Cut{(Tile)t, splits, per * K, us};
     }
   }
