@@ -639,9 +639,11 @@ struct Cut {
 // workgroup, at the time a load takes; for a split sum the second launch, and the parts written and read.  The constants
 // are fitted to 160 products of 1 to 10^6 rows and 24 to 4096 columns, forward and the three backward ones, bf16 and
 // float32, each measured in all cuts: the choice is 2 % slower than the best cut on average, 29 % at worst (14 us for 11).
+// ANY64's are from nine odd products (a stage of 2.2 to 6.4 us alone and 2 to 3.5 shared, in either type): 1000 x 2001 -> 1001
+// in bf16 takes 132 us there and 27 as padded copies, 25 x 1087 -> 15 in float32 75 and 15; 4 x 25 -> 678 stays at 6.
 Cut pick_cut(int esize, bool staged, int64_t p, int64_t q, int64_t r) {
   struct Rate { double full, alone, per_output; int at_a_time; };
-  static const Rate rates[] = {{0.8, 1.2, 3e-5, 3}, {0.057, 0.45, 3e-5, 3}, {0.41, 0.745, 3e-5, 2}, {1.06, 0.2, 7e-5, 1}};   // by Tile
+  static const Rate rates[] = {{2.5, 4.0, 3e-5, 3}, {0.057, 0.45, 3e-5, 3}, {0.41, 0.745, 3e-5, 2}, {1.06, 0.2, 7e-5, 1}};   // by Tile
   const int K = ROW_BYTES / esize;
   const int64_t stages = (r + K - 1) / K;
   Cut best{ANY64, 1, stages * K, 1e300};
@@ -649,7 +651,7 @@ Cut pick_cut(int esize, bool staged, int64_t p, int64_t q, int64_t r) {
     const int edge = tile_edge((Tile)t), slots = 256 * rates[t].at_a_time;
     const int64_t tiles = (int64_t)cdiv(p, edge) * cdiv(q, edge);
     auto round_us = [&](int64_t wgs, int64_t per) {
-      const double share = wgs > 256 ? wgs / 256.0 : 1.0, full = rates[t].full * (esize == 4 ? 1.84 : 1.0) * share;
+      const double share = wgs > 256 ? wgs / 256.0 : 1.0, full = rates[t].full * (esize == 4 && t != ANY64 ? 1.84 : 1.0) * share;
       return 2.6 + rates[t].per_output * edge * edge * share + per * (full > rates[t].alone ? full : rates[t].alone);
     };
     for (int s = 1; s <= 1024; s *= 2) {
