@@ -12,6 +12,8 @@
 // The statistics are plain sums of x and x*x in 64 bits: on this chip a double add costs what a float add costs,
 // and 53 bits make the subtraction E[x^2] - mean^2 harmless (any spread that the input's 24 bits can hold survives).
 // Sums over pixels are combined in a fixed order: results repeat bit for bit.
+#include <algorithm>
+
 #include "act.h"
 #include "common.h"
 
@@ -776,16 +778,26 @@ template <int MOST, typename F> void with_count(int n, F&& f) {
   else f(std::integral_constant<int, MOST>());
 }
 
-int resident_grid(const Shape& s, int B) { return (B * s.slabs + 7) / 8 * 8; }
+// f(first sample, samples, workgroups) for each launch: a launch has 2^22 slabs at most (a launch holds below 2^32 threads).
+template <typename F> void by_samples(const Shape& s, int B, F&& f) {
+  const int most = std::max(1, (1 << 22) / s.slabs);
+  for (int b = 0; b < B; b += most) {
+    const int n = std::min(most, B - b);
+    f((int64_t)b, n, (n * s.slabs + 7) / 8 * 8);
+  }
+}
 
 template <typename T, int V>
 void launch_resident_fwd(const T* x, const Shape& s, int nv, int B, const float* gamma, const float* beta, double eps, int act,
                          T* y, double2* stats, hipStream_t st) {
-  const int grid = resident_grid(s, B);
+  const int64_t sample = s.HW * s.C;
   with_act(act, [&](auto a) {
     constexpr int ACT = decltype(a)::value;
     with_count<RES_FWD>(nv, [&](auto n) {
-      gn_resident_kernel<T, V, decltype(n)::value, ACT><<<grid, RES_THREADS, 0, st>>>(x, s, B, eps, gamma, beta, y, stats);
+      by_samples(s, B, [&](int64_t b, int nb, int grid) {
+        gn_resident_kernel<T, V, decltype(n)::value, ACT><<<grid, RES_THREADS, 0, st>>>(
+            x + b * sample, s, nb, eps, gamma, beta, y + b * sample, stats + b * s.G);
+      });
     });
   });
 }
@@ -793,11 +805,15 @@ void launch_resident_fwd(const T* x, const Shape& s, int nv, int B, const float*
 template <typename T, int V>
 void launch_resident_bwd(const T* x, const T* dy, const Shape& s, int nv, int B, const float* gamma, const float* beta, int act,
                          const double2* stats, T* dx, float* dgamma, float* dbeta, float* chan, hipStream_t st) {
-  const int grid = resident_grid(s, B);
+  const int64_t sample = s.HW * s.C;
   with_act(act, [&](auto a) {
     constexpr int ACT = decltype(a)::value;
     with_count<RES_BWD>(nv, [&](auto n) {
-      gn_resident_bwd_kernel<T, V, decltype(n)::value, ACT><<<grid, RES_THREADS, 0, st>>>(x, dy, s, B, stats, gamma, beta, dx, chan);
+      by_samples(s, B, [&](int64_t b, int nb, int grid) {
+        gn_resident_bwd_kernel<T, V, decltype(n)::value, ACT><<<grid, RES_THREADS, 0, st>>>(
+            x + b * sample, dy + b * sample, s, nb, stats + b * s.G, gamma, beta, dx ? dx + b * sample : nullptr,
+            chan + b * 2 * s.C);
+      });
     });
   });
   if (dgamma || dbeta)
@@ -900,9 +916,9 @@ size_t mis_group_norm_act_fwd_workspace_bytes(int dtype, int B, int64_t HW, int 
 
 int mis_group_norm_act_fwd(const void* x, int dtype, int B, int64_t HW, int C, int G, const float* gamma, const float* beta,
                            double eps, int act, void* y, double* stats, void* workspace, mis_stream_t stream) {
-  MIS_REQUIRE(x && y && stats && workspace, "group_norm_act_fwd: null pointer");
   MIS_REQUIRE(shape_ok(dtype, B, HW, C, G), "group_norm_act_fwd: bad dtype or shape (B=%d HW=%lld C=%d groups=%d)", B,
               (long long)HW, C, G);
+  MIS_REQUIRE(x && y && stats && workspace, "group_norm_act_fwd: null pointer");
   MIS_REQUIRE(act >= MIS_ACT_NONE && act <= MIS_ACT_GELU, "group_norm_act_fwd: unknown activation %d", act);
   MIS_REQUIRE(eps >= 0.0, "group_norm_act_fwd: eps must not be negative");
   MIS_REQUIRE((((uintptr_t)x | (uintptr_t)y) & (dtype == MIS_BF16 ? 1 : 3)) == 0 &&
@@ -934,9 +950,9 @@ size_t mis_group_norm_act_bwd_workspace_bytes(int dtype, int B, int64_t HW, int 
 int mis_group_norm_act_bwd(const void* x, const void* dy, int dtype, int B, int64_t HW, int C, int G, const float* gamma,
                            const float* beta, const double* stats, int act, void* dx, float* dgamma, float* dbeta,
                            void* workspace, mis_stream_t stream) {
-  MIS_REQUIRE(x && dy && stats && workspace, "group_norm_act_bwd: null pointer");
   MIS_REQUIRE(shape_ok(dtype, B, HW, C, G), "group_norm_act_bwd: bad dtype or shape (B=%d HW=%lld C=%d groups=%d)", B,
               (long long)HW, C, G);
+  MIS_REQUIRE(x && dy && stats && workspace, "group_norm_act_bwd: null pointer");
   MIS_REQUIRE(act >= MIS_ACT_NONE && act <= MIS_ACT_GELU, "group_norm_act_bwd: unknown activation %d", act);
   MIS_REQUIRE((((uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx) & (dtype == MIS_BF16 ? 1 : 3)) == 0 &&
               (((uintptr_t)stats | (uintptr_t)workspace) & 15) == 0, "group_norm_act_bwd: misaligned pointer");

@@ -787,7 +787,8 @@ template <typename T> struct Buffers {
 
 bool sizes_ok(int dtype, int64_t M, int64_t N, int64_t K) {
   return (dtype == MIS_F32 || dtype == MIS_BF16) && M >= 1 && N >= 1 && K >= 1 && N <= 1 << 20 && K <= 1 << 20 &&
-         M < ((int64_t)1 << 30) && (M + 63) / 64 * ((N > K ? N : K) + 63) / 64 < ((int64_t)1 << 31);
+         M < ((int64_t)1 << 30) &&
+         (M + 63) / 64 * (((N > K ? N : K) + 63) / 64) <= (1 << 24) - 8;      // tiles of 256 threads: a launch holds below 2^32
 }
 
 bool aligned(int dtype, std::initializer_list<const void*> ps) {
@@ -889,9 +890,9 @@ size_t mis_linear_act_fwd_workspace_bytes(int dtype, int64_t M, int64_t N, int64
 
 int mis_linear_act_fwd(const void* x, int64_t ldx, const void* w, const float* bias, const void* residual, int64_t ldr, int dtype,
                        int64_t M, int64_t N, int64_t K, int act, void* y, void* workspace, mis_stream_t stream) {
-  MIS_REQUIRE(x && w && y && workspace, "linear_act_fwd: null pointer");
   MIS_REQUIRE(sizes_ok(dtype, M, N, K), "linear_act_fwd: bad dtype or sizes (M=%lld N=%lld K=%lld)", (long long)M, (long long)N,
               (long long)K);
+  MIS_REQUIRE(x && w && y && workspace, "linear_act_fwd: null pointer");
   MIS_REQUIRE(ldx >= K && (!residual || ldr >= N), "linear_act_fwd: row stride below the row length");
   MIS_REQUIRE(act >= MIS_ACT_NONE && act <= MIS_ACT_GELU, "linear_act_fwd: unknown activation %d", act);
   MIS_REQUIRE(aligned(dtype, {x, w, residual, y}) && ((uintptr_t)workspace & 15) == 0, "linear_act_fwd: misaligned pointer");
@@ -916,9 +917,9 @@ size_t mis_linear_act_bwd_workspace_bytes(int dtype, int64_t M, int64_t N, int64
 int mis_linear_act_bwd(const void* x, int64_t ldx, const void* w, const float* bias, const void* dy, int64_t ldd, int dtype,
                        int64_t M, int64_t N, int64_t K, int act, void* dx, void* dw, float* db, void* workspace,
                        mis_stream_t stream) {
-  MIS_REQUIRE(x && w && dy && workspace, "linear_act_bwd: null pointer");
   MIS_REQUIRE(sizes_ok(dtype, M, N, K), "linear_act_bwd: bad dtype or sizes (M=%lld N=%lld K=%lld)", (long long)M, (long long)N,
               (long long)K);
+  MIS_REQUIRE(x && w && dy && workspace, "linear_act_bwd: null pointer");
   MIS_REQUIRE(ldx >= K && ldd >= N, "linear_act_bwd: row stride below the row length");
   MIS_REQUIRE(act >= MIS_ACT_NONE && act <= MIS_ACT_GELU, "linear_act_bwd: unknown activation %d", act);
   MIS_REQUIRE(aligned(dtype, {x, w, dy, dx, dw}) && ((uintptr_t)workspace & 15) == 0, "linear_act_bwd: misaligned pointer");

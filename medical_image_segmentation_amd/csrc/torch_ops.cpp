@@ -58,6 +58,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
     c10::DeviceGuard guard(x.device());
     const Tensor w = dense(weight), b = dense(bias);
     const int64_t B = x.size(0), C = x.size(1), HW = x.size(2) * x.size(3);
+    TORCH_CHECK(B <= INT32_MAX && C <= INT32_MAX, "group_norm_act: ", B, " samples of ", C, " channels are too many");
     Tensor y = at::empty_like(x, at::MemoryFormat::ChannelsLast);
     Tensor stats = at::empty({B, groups, 2}, x.options().dtype(at::kDouble));
     if (x.numel()) {

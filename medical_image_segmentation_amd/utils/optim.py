@@ -131,7 +131,7 @@ def clip_and_step(optimizer, params, max_norm=1.0):
     if isinstance(optimizer, AdamW8):
         stepped, given = optimizer._stepped(), [p for p in params if p.grad is not None]
         same = len(stepped) == len(given) and all(map(operator.is_, stepped, given))
-        if not same and {id(p) for p in given} != {id(p) for p in stepped}:
+        if not same and (len(stepped) != len(given) or {id(p) for p in given} != {id(p) for p in stepped}):
             norm = torch.nn.utils.clip_grad_norm_(params, max_norm=max_norm)   # a norm over other tensors than are stepped
             optimizer.step()
             return norm
@@ -289,6 +289,9 @@ class AdamW8(torch.optim.Optimizer):
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
+        if len({id(p) for p in self.param_groups[-1]["params"]}) != len(self.param_groups[-1]["params"]):
+            self.param_groups.pop()
+            raise ValueError("AdamW8 takes each parameter once: all of them are updated by one launch")
         for p in self.param_groups[-1]["params"]:
             if p.dtype not in F_._DT:
                 self.param_groups.pop()
@@ -473,6 +476,9 @@ class _Table8:
         return out, keep
 
     def rows(self, pointers):
+        spans = sorted((pointers[2 * i], pointers[2 * i] + p.nbytes) for i, p in enumerate(self.order))
+        if any(end > begin for (_, end), (begin, _) in zip(spans, spans[1:])):
+            raise RuntimeError("AdamW8 updates all parameters in one launch: two of them share memory")
         return [(pointers[2 * i], pointers[2 * i + 1], *f) for i, f in enumerate(self.fixed)]
 
     def refresh(self):
@@ -544,9 +550,10 @@ class _CapturedStep8:
             b1, b2 = g["betas"]
             call("mis_adamw8_step_constants", float(g["lr"]), float(b1), float(b2), float(g["weight_decay"]),
                  self.table.states[k][0]["step"] + 1, host[k].data_ptr())
-        self.dyn.copy_(host, non_blocking=True)
-        ev = torch.cuda.Event()
-        ev.record()
+        with F_._on_device_of(self.dyn):
+            self.dyn.copy_(host, non_blocking=True)
+            ev = torch.cuda.Event()
+            ev.record()
         self.dyn_done[i] = ev
 
     def launch(self):

@@ -40,10 +40,11 @@ def linear_act64(x, weight, bias, act, residual):
 # ---------------------------------------------------------------------------------------------------------------
 # AdamW8
 # ---------------------------------------------------------------------------------------------------------------
-def philox(n, step, seed):
-    """n 32-bit words, word i from the counter (i // 4, step) under the key `seed`."""
+def philox(n, step, seed, first=0):
+    """n 32-bit words from the word `first` (a multiple of 4) on, word i from the counter (i // 4, step) under the key
+    `seed`."""
     u = np.uint64
-    i = np.arange((n + 3) // 4, dtype=np.uint64)
+    i = np.arange((n + 3) // 4, dtype=np.uint64) + u(first // 4)
     m32 = u(0xFFFFFFFF)
     c = [i & m32, i >> u(32), np.full_like(i, step & 0xFFFFFFFF), np.full_like(i, step >> 32)]
     k0, k1 = seed & 0xFFFFFFFF, seed >> 32

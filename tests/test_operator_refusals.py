@@ -102,3 +102,22 @@ def test_adamw8_refusals():
         opt.load_state_dict({"state": {0: {**codes, "exp_avg_scale": torch.zeros(1)}}, "param_groups": groups})
     opt.load_state_dict({"state": {0: codes}, "param_groups": groups})
     assert opt.state[p]["step"] == 3 and opt.state[p]["exp_avg"].dtype == torch.uint8
+
+
+def test_adamw8_takes_a_parameter_once():
+    from medical_image_segmentation_amd.utils.optim import AdamW8
+    p, q = torch.nn.Parameter(torch.zeros(4)), torch.nn.Parameter(torch.zeros(4))
+    with pytest.warns(UserWarning), pytest.raises(ValueError, match="takes each parameter once"):
+        AdamW8([p, q, p])
+    opt = AdamW8([p])
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=[p]))
+    assert len(opt.param_groups) == 1
+
+
+def test_grids_that_no_launch_holds():
+    """2^30 rows of one column would need 2^24 tiles of 256 threads; a launch holds below 2^32 threads."""
+    from medical_image_segmentation_amd._lib import query
+    assert query("mis_linear_act_fwd_workspace_bytes", 1, (1 << 30) - 1, 1, 1) == 0
+    assert query("mis_linear_act_fwd_workspace_bytes", 1, ((1 << 24) - 8) * 64, 1, 1) > 0
+    _refused("mis_linear_act_fwd", P, 1, P, None, None, 1, 1, (1 << 30) - 1, 1, 1, 0, P, P, None, match="bad dtype or sizes")
