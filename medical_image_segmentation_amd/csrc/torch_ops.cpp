@@ -6,6 +6,7 @@
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -35,6 +36,21 @@ struct Wanted {
 void check(int rc, const char* name) {
   TORCH_CHECK(rc == MIS_OK, name, " failed (status ", rc, "): ", mis_last_error());
 }
+
+// A backward pass under capture must not reach a leaf whose gradient node was made on the default stream, which cannot join
+// a capture: the node lives as long as any graph that uses the leaf, here one from before the capture.  (The engine would
+// wait on that stream at the end of the pass and the capture would end with the process.)
+void refuse_stale_leaf(const Tensor& t, bool capturing, const char* name) {
+  if (!capturing || !t.defined() || !t.requires_grad() || !t.is_leaf()) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!node) return;
+  const auto made_on = node->stream();
+  TORCH_CHECK(!made_on || made_on->id() != c10::hip::getDefaultHIPStream(t.get_device()).id(), name,
+              ": an eager graph of the same leaf is alive; drop the tensors that hold it (outputs, losses) before capturing a "
+              "backward pass");
+}
+
+bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
 
 // Gradients that raise when they are differentiated with respect to what they were formed from: the backward is not
 // differentiable itself.
@@ -79,6 +95,8 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
     const bool twice = at::GradMode::is_enabled();         // create_graph=True
     at::NoGradGuard no_grad;
     c10::DeviceGuard guard(x.device());
+    const bool captured = capturing();
+    for (const Tensor& t : {x, w, b}) refuse_stale_leaf(t, captured, "group_norm_act");
     const int64_t B = x.size(0), C = x.size(1), HW = x.size(2) * x.size(3);
     const bool some = x.numel() > 0;
     Tensor dx, dw, db;
@@ -137,6 +155,8 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     const bool twice = at::GradMode::is_enabled();         // create_graph=True
     at::NoGradGuard no_grad;
     c10::DeviceGuard guard(x.device());
+    const bool captured = capturing();
+    for (const Tensor& t : {x, w, b}) refuse_stale_leaf(t, captured, "linear_act");
     const int64_t N = w.size(0), K = w.size(1), M = x.numel() / K;
     Tensor dx, dw, db, dr;
     Wanted wanted{ctx};

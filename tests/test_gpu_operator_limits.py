@@ -171,3 +171,33 @@ def test_the_same_tensor_in_every_place():
     ref.linear_act64(r, r, None, "silu", r).backward(torch.ones(48, 48, device=DEV, dtype=torch.float64))
     # 96 terms of products of |t| < 5 per element, each off by at most 48 roundings of the sum: 1e-5 of the whole
     assert float((t.grad - r.grad).norm() / r.grad.norm()) < 1e-5
+
+
+@pytest.mark.parametrize("op", ["group_norm_act", "linear_act"])
+def test_captured_backward_refuses_leaves_of_a_living_eager_graph(op):
+    """The gradient node of a leaf that an eager graph on the default stream keeps alive cannot take part in a capture."""
+    from medical_image_segmentation_amd import functional as F_
+    w = torch.ones(32, device=DEV, requires_grad=True)
+    m = torch.randn(32, 32, device=DEV, requires_grad=True)
+    x = torch.randn(2, 32, 6, 6, device=DEV).contiguous(memory_format=torch.channels_last)
+    leaf = w if op == "group_norm_act" else m
+    run = lambda: F_.group_norm_act(x, 4, w) if op == "group_norm_act" else F_.pointwise_conv_act(x, m)  # noqa: E731
+    alive = run()
+    (want,) = torch.autograd.grad(alive, [leaf], torch.ones_like(alive), retain_graph=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph of the same leaf is alive"):
+        with torch.cuda.graph(graph):
+            y = run()
+            torch.autograd.grad(y, [leaf], torch.ones_like(y))
+    del alive, y
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = run()
+        (got,) = torch.autograd.grad(y, [leaf], torch.ones_like(y))
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
