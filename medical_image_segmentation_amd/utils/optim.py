@@ -307,12 +307,20 @@ class AdamW8(torch.optim.Optimizer):
                 want = _blocks(n[i]) * (1 if k.endswith("_scale") else BLOCK8) if i in n else None
                 if want is not None and (s[k].dtype != torch.uint8 or s[k].numel() != want):
                     raise ValueError(f"parameter {i}: {k} should be {want} bytes, got {s[k].numel()} of {s[k].dtype}")
-        super().load_state_dict(state_dict)        # (casts to the parameter's type, which holds 0..255 exactly)
-        for s in self.state.values():
-            for k in self._STATE:
-                s[k] = s[k].to(torch.uint8).reshape(-1)
-            s["step"] = int(s["step"])
+        # (the codes go past torch's loading, which would take them through the parameters' floating-point type)
+        states = state_dict["state"]
+        rest = {i: {k: v for k, v in s.items() if k not in self._STATE} for i, s in states.items()}
+        super().load_state_dict({**state_dict, "state": rest})
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip((i for g in state_dict["param_groups"] for i in g["params"]), params):
+            if i in states:
+                self.state[p].update({k: states[i][k].reshape(-1) for k in self._STATE}, step=int(states[i]["step"]))
         self._plan = None
+        if all(p.is_cuda for p in params) and len({p.device for p in params}) == 1:
+            self._flat()
+        else:                                      # nothing of the given tensors is kept
+            for s in self.state.values():
+                s.update({k: s[k].clone() for k in self._STATE if k in s})
 
     def _stepped(self):
         return [p for g in self.param_groups for p in g["params"] if p.grad is not None]
@@ -327,16 +335,20 @@ class AdamW8(torch.optim.Optimizer):
         if len(devs) != 1 or next(iter(devs)).type != "cuda":
             raise RuntimeError(f"AdamW8 needs all parameters on one GPU, got {sorted(map(str, devs))}")
         plan = self._plan = _Plan8(params, next(iter(devs)))
-        for p, (b0, b1) in zip(params, plan.spans):
-            s, old = self.state[p], dict(self.state[p])
-            for k, buf in zip(self._STATE, plan.buffers):
-                w = 1 if k.endswith("_scale") else BLOCK8
-                s[k] = buf[b0 * w:b1 * w]
-                if k in old:
-                    s[k].copy_(old[k])
-                    if w == BLOCK8:
-                        s[k][p.numel():].zero_()
-            s["step"] = int(old.get("step", 0))
+        views = [buf.split([(b1 - b0) * w for b0, b1 in plan.spans] + [buf.numel() - plan.blocks * w])
+                 for buf, w in zip(plan.buffers, (BLOCK8, 1, BLOCK8, 1))]
+        to, given = [], []
+        for i, p in enumerate(params):
+            s = self.state[p]
+            for k, v in zip(self._STATE, views):
+                if k in s:                        # (codes behind the last element stay zero)
+                    n = p.numel() if v is views[0] or v is views[2] else v[i].numel()
+                    to.append(v[i][:n])
+                    given.append(s[k][:n])
+                s[k] = v[i]
+            s["step"] = int(s.get("step", 0))
+        if to:
+            torch._foreach_copy_(to, given)
         return plan
 
     def moments(self, p=None):

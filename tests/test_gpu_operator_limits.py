@@ -216,3 +216,40 @@ def test_captured_backward_refuses_leaves_of_a_living_eager_graph(op):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+def test_adamw8_loads_a_state_from_the_host_and_keeps_nothing_of_it():
+    import io
+    from medical_image_segmentation_amd.utils.optim import AdamW8
+
+    def make():
+        g = torch.Generator().manual_seed(5)
+        ps = [torch.nn.Parameter((torch.randn(n, generator=g) * 0.1).to(DEV)) for n in (300, 0, 128, 4097)]
+        for p in ps:
+            p.grad = torch.full_like(p, 1e-2)
+        return ps, AdamW8(ps, lr=1e-2, seed=9)
+
+    pa, oa = make()
+    oa.step()
+    file = io.BytesIO()
+    torch.save(oa.state_dict(), file)
+    file.seek(0)
+    pb, ob = make()
+    with torch.no_grad():
+        for p, q in zip(pb, pa):
+            p.copy_(q)
+    state = torch.load(file, map_location="cpu", weights_only=True)
+    state["state"][0]["exp_avg"][300:] = 77              # codes behind the last element mean nothing
+    ob.load_state_dict(state)
+    pc, oc = make()
+    with torch.no_grad():
+        for p, q in zip(pc, pa):
+            p.copy_(q)
+    oc.load_state_dict(oa.state_dict())                  # the live buffers of another optimizer
+    oa.step(), ob.step(), oc.step()
+    for a, b, c in zip(pa, pb, pc):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    for k in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"):
+        for a, b, c in zip(pa, pb, pc):
+            assert torch.equal(oa.state[a][k], ob.state[b][k]) and torch.equal(oa.state[a][k], oc.state[c][k])
+    assert [oc.state[p]["step"] for p in pc] == [2, 2, 2, 2]
