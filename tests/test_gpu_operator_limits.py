@@ -253,3 +253,39 @@ def test_adamw8_loads_a_state_from_the_host_and_keeps_nothing_of_it():
         for a, b, c in zip(pa, pb, pc):
             assert torch.equal(oa.state[a][k], ob.state[b][k]) and torch.equal(oa.state[a][k], oc.state[c][k])
     assert [oc.state[p]["step"] for p in pc] == [2, 2, 2, 2]
+
+
+def test_two_threads_on_two_streams():
+    """The same block trained from two threads at once, each with its own stream and optimizer: the results of one alone."""
+    import threading
+    from medical_image_segmentation_amd.model.utils.modules import ChannelMLP
+    from medical_image_segmentation_amd.utils.optim import AdamW8, clip_and_step
+
+    def train(seed, out):
+        g = torch.Generator().manual_seed(seed)
+        m = ChannelMLP(32, num_groups=4)
+        with torch.no_grad():
+            for p in m.parameters():
+                p.copy_(torch.randn(p.shape, generator=g) * 0.1)
+        xs = [torch.randn(2, 32, 24, 20 + seed, generator=g) for _ in range(5)]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            m.to(DEV)
+            opt = AdamW8(m.parameters(), lr=1e-2, seed=seed)
+            for x in xs:
+                opt.zero_grad()
+                m(x.to(DEV)).square().mean().backward()
+                clip_and_step(opt, m.parameters(), 0.5)
+            torch.cuda.current_stream().synchronize()
+        out[seed] = [p.detach().clone() for p in m.parameters()]
+        torch.cuda.synchronize()
+
+    alone, both = {}, {}
+    for s in (1, 2):
+        train(s, alone)
+    threads = [threading.Thread(target=train, args=(s, both)) for s in (1, 2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for s in (1, 2):
+        assert all(torch.equal(a, b) for a, b in zip(alone[s], both[s]))
