@@ -650,7 +650,8 @@ int mis_group_norm_act_bwd(const void* x, const void* dy, int dtype, int B, int6
 /* The backward forms u = x W^T + b again (only if act is not MIS_ACT_NONE):        */
 /*   dz = dy act'(u);  dx = dz W;  dw = dz^T x;  db = sum over rows of dz           */
 /* (dr is dy).  dx, dw dense in the element type, db float32; each may be NULL.     */
-/* dy has row stride ldd.  M < 2^30, N and K <= 2^20.                               */
+/* dy has row stride ldd.  M < 2^30, N and K <= 2^20, and ceil(M / 64) *            */
+/* ceil(max(N, K) / 64) <= 2^24 - 8.                                               */
 size_t mis_linear_act_fwd_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
 int mis_linear_act_fwd(const void* x, int64_t ldx, const void* w, const float* bias, const void* residual, int64_t ldr, int dtype,
                        int64_t M, int64_t N, int64_t K, int act, void* y, void* workspace, mis_stream_t stream);
