@@ -31,7 +31,7 @@ __device__ __forceinline__ float act_value(float u) {
   } else if constexpr (ACT == MIS_ACT_GELU) {
     float q, e;                                  // u Phi(u) = max(u, 0) - |u| Phi(-|u|)
     gelu_parts(u, q, e);
-    return fmaf(-fabsf(fminf(u, 64.f)), q, u < 0.f ? 0.f : u);       // (q is zero from there on, also at infinity)
+    return fmaf(-fabsf(fminf(u, 64.f)), q, fmaxf(u, 0.f));       // (q is 0 from 64 on, also at infinity; NaN for NaN)
   } else {
     return u;
   }
