@@ -185,6 +185,35 @@ Tensor linear_act(const Tensor& x, const Tensor& weight, const Maybe& bias, cons
   return LinearAct::apply(x, weight, bias, residual, act);
 }
 
+// The types, devices, shapes and strides of parameters: what an optimizer's tables of them hold good for.  A Parameter stays
+// the same object when its module is converted (Module.to, .bfloat16) or its .data replaced, so these are compared at every
+// step; in C++, since the interpreter would take as long for it as the step's launches.
+class Layouts {
+ public:
+  explicit Layouts(std::vector<Tensor> params) : params_(std::move(params)) {
+    for (const Tensor& p : params_) kept_.push_back({p.scalar_type(), p.device(), p.sizes().vec(), p.strides().vec()});
+  }
+  bool hold() const {
+    for (size_t i = 0; i < params_.size(); i++) {
+      const Tensor& p = params_[i];
+      const One& k = kept_[i];
+      if (p.scalar_type() != k.type || p.device() != k.device || p.sizes() != at::IntArrayRef(k.sizes) ||
+          p.strides() != at::IntArrayRef(k.strides))
+        return false;
+    }
+    return true;
+  }
+
+ private:
+  struct One {
+    at::ScalarType type;
+    at::Device device;
+    std::vector<int64_t> sizes, strides;
+  };
+  std::vector<Tensor> params_;
+  std::vector<One> kept_;
+};
+
 // The pointers [parameter, gradient, parameter, ...] of parameters whose gradients lie in the same memory order, type and
 // device; empty if one does not (the caller then looks at them one by one).
 std::vector<int64_t> step_pointers(const std::vector<Tensor>& params, int64_t device) {
@@ -193,7 +222,7 @@ std::vector<int64_t> step_pointers(const std::vector<Tensor>& params, int64_t de
   for (const Tensor& p : params) {
     const Tensor& g = p.grad();
     if (!g.defined() || g.is_sparse() || g.scalar_type() != p.scalar_type() || g.get_device() != device ||
-        p.get_device() != device || !(g.is_contiguous() && p.is_contiguous()))
+        p.get_device() != device || !(g.is_contiguous() && p.is_contiguous()) || g.sizes() != p.sizes())
       return {};
     out.push_back((int64_t)p.data_ptr());
     out.push_back((int64_t)g.data_ptr());
@@ -207,4 +236,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("group_norm_act", &group_norm_act, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("linear_act", &linear_act, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("step_pointers", &step_pointers);
+  pybind11::class_<Layouts>(m, "Layouts").def(pybind11::init<std::vector<Tensor>>()).def("hold", &Layouts::hold);
 }

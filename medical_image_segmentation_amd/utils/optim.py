@@ -258,6 +258,20 @@ def _dense(t):
     return True
 
 
+def _layout(p):
+    """(shape, dimensions by falling stride): which element lies at which place of a dense tensor's memory."""
+    dims = [d for d in range(p.dim()) if p.shape[d] != 1] if p.numel() else []
+    return tuple(p.shape), tuple(sorted(dims, key=lambda d: -p.stride(d)))
+
+
+def _check_layout(i, p, s):
+    """The codes of state `s` follow the memory of the tensor they were made for: they mean nothing in another order."""
+    if "layout" in s and s["layout"] != _layout(p):
+        raise RuntimeError(f"AdamW8: parameter {i} is now {tuple(p.shape)} with strides {p.stride()}, its moments were made for "
+                           f"shape {s['layout'][0]} with the dimensions {s['layout'][1]} by falling stride: convert the model "
+                           "back, or delete the parameter's state to begin again")
+
+
 class AdamW8(torch.optim.Optimizer):
     """AdamW with both moments in 8 bits, one launch for all tensors (two when the gradient norm is clipped).
 
@@ -268,8 +282,11 @@ class AdamW8(torch.optim.Optimizer):
     that is not finite makes its block of 128 read back as NaN.
 
     state[p] = {"step": int, "exp_avg", "exp_avg_sq": uint8 codes, padded to a multiple of 128,
-                "exp_avg_scale", "exp_avg_sq_scale": uint8, one per 128}; `moments(p)` gives their float32 values.
-    The codes follow the elements' order in memory.  A parameter without a gradient is left alone, as in torch.
+                "exp_avg_scale", "exp_avg_sq_scale": uint8, one per 128,
+                "layout": (shape, dimensions by falling stride)}; `moments(p)` gives their float32 values.
+    The codes follow the elements' order in memory.  A parameter may change its type, device or address between steps
+    (Module.bfloat16(), .data = ...), but not its shape or memory order: the step raises then.  A parameter without a
+    gradient is left alone, as in torch.
     """
     _STATE = ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale")
     _plan = None
@@ -334,6 +351,8 @@ class AdamW8(torch.optim.Optimizer):
         devs = {p.device for p in params}
         if len(devs) != 1 or next(iter(devs)).type != "cuda":
             raise RuntimeError(f"AdamW8 needs all parameters on one GPU, got {sorted(map(str, devs))}")
+        for i, p in enumerate(params):
+            _check_layout(i, p, self.state.get(p, {}))
         plan = self._plan = _Plan8(params, next(iter(devs)))
         views = [buf.split([(b1 - b0) * w for b0, b1 in plan.spans] + [buf.numel() - plan.blocks * w])
                  for buf, w in zip(plan.buffers, (BLOCK8, 1, BLOCK8, 1))]
@@ -347,6 +366,7 @@ class AdamW8(torch.optim.Optimizer):
                     given.append(s[k][:n])
                 s[k] = v[i]
             s["step"] = int(s.get("step", 0))
+            s["layout"] = _layout(p)
         if to:
             torch._foreach_copy_(to, given)
         return plan
@@ -401,6 +421,8 @@ class _Plan8:
         self.params, self.device = params, device
         self.spans, at = [], 0
         for p in params:
+            if p.dtype not in F_._DT:
+                raise TypeError(f"AdamW8 takes float32 and bfloat16 parameters, got {p.dtype}")
             if not _dense(p):
                 raise RuntimeError(f"AdamW8 needs dense parameters, got strides {p.stride()} for {tuple(p.shape)}")
             self.spans.append((at, at + _blocks(p.numel())))
@@ -408,10 +430,12 @@ class _Plan8:
         self.blocks = at
         self.buffers = [torch.zeros(max(at, 1) * w, dtype=torch.uint8, device=device) for w in (BLOCK8, 1, BLOCK8, 1)]
         self.norm_ws = torch.empty(query("mis_adamw8_workspace_bytes"), dtype=torch.uint8, device=device)
+        self.layouts = F_._native().Layouts(params)
         self.tables = []
 
     def matches(self, params):
-        return len(params) == len(self.params) and all(map(operator.is_, params, self.params))
+        """Whether these are the parameters that buffers and tables were made for, in type, device, shape and strides too."""
+        return len(params) == len(self.params) and all(map(operator.is_, params, self.params)) and self.layouts.hold()
 
     def table(self, groups, state, params):
         """The launch tables for `params`, the parameters that have a gradient now."""
@@ -478,9 +502,9 @@ class _Table8:
             return out, keep
         for p, plain, dtype in zip(self.order, self.plain, self.dtypes):
             g = p.grad
-            if g.dtype is not dtype or g.is_sparse or g.get_device() != dev or p.get_device() != dev:
-                raise RuntimeError(f"AdamW8 needs dense gradients of the parameter's type and device, got {g.dtype} "
-                                   f"{g.layout} on {g.device} for {p.dtype} on {p.device}")
+            if g.dtype is not dtype or g.is_sparse or g.get_device() != dev or p.get_device() != dev or g.shape != p.shape:
+                raise RuntimeError(f"AdamW8 needs dense gradients of the parameter's type, device and shape, got {g.dtype} "
+                                   f"{g.layout} {tuple(g.shape)} on {g.device} for {p.dtype} {tuple(p.shape)} on {p.device}")
             if not (plain and g.is_contiguous()) and g.stride() != p.stride():
                 g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g.detach())
                 keep.append(g)
@@ -538,6 +562,7 @@ class _CapturedStep8:
                                "(clip_and_step)")
         self.plan = optimizer._flat()
         self.table = _Table8(self.plan, optimizer.param_groups, optimizer.state, self.params)
+        self.addresses = [p.data_ptr() for p in self.table.order]
         dev, n, r = self.plan.device, len(self.table.order), max(len(self.table.runs), 1)
         self.rows_host = torch.empty((n, 5), dtype=torch.int64).pin_memory()
         self.descs = torch.empty((n, 5), dtype=torch.int64, device=dev)
@@ -551,6 +576,8 @@ class _CapturedStep8:
     def prepare(self):
         if self.optimizer._plan is not self.plan:
             raise RuntimeError("the optimizer's state was replaced after the capture")
+        if not self.plan.matches(self.plan.params) or [p.data_ptr() for p in self.table.order] != self.addresses:
+            raise RuntimeError("a parameter was converted or its memory replaced after the capture: capture the step again")
         if not self.table.serves(self.params):
             raise RuntimeError("the parameters' step numbers no longer agree: capture the step again")
         i = self.slot
@@ -570,6 +597,7 @@ class _CapturedStep8:
 
     def launch(self):
         pointers, self.keep = self.table.addresses()
+        self.addresses = pointers[::2]                          # the parameters', which every replay writes to
         self.rows_host.copy_(torch.tensor(self.table.rows(pointers), dtype=torch.int64))
         self.descs.copy_(self.rows_host, non_blocking=True)
         self.norm = self.table.launch(self.max_norm, self.descs, self.ws, self.dyn)

@@ -1,0 +1,91 @@
+"""CPU suite: what AdamW8 keeps from one step to the next, and when it may not be used any more."""
+import pytest
+import torch
+
+
+def _params(*shapes):
+    g = torch.Generator().manual_seed(1)
+    return [torch.nn.Parameter(torch.randn(s, generator=g)) for s in shapes]
+
+
+def _converted():
+    """(what is done, whether the moments' codes still fit) for a parameter [6, 4, 3, 3] that stays the same object."""
+    def typed(p):
+        p.data = p.data.bfloat16()
+
+    def order(p):
+        p.data = p.data.contiguous(memory_format=torch.channels_last)
+
+    def fewer(p):
+        p.data = p.data[:3].contiguous()
+
+    def shape(p):
+        p.data = p.data.reshape(4, 6, 3, 3)
+
+    def transposed(p):
+        p.data = p.data.transpose(0, 1)
+
+    return [(typed, True), (order, False), (fewer, False), (shape, False), (transposed, False)]
+
+
+@pytest.mark.parametrize("change,fits", _converted())
+def test_tables_of_a_converted_parameter_are_not_used_again(change, fits):
+    """The kernels take a tensor's address, length and type from these tables: with those of another type or length they would
+    read and write behind its end."""
+    from medical_image_segmentation_amd.utils.optim import _Plan8, _check_layout, _layout
+    params = _params((5,), (6, 4, 3, 3), (0,))
+    plan = _Plan8(params, torch.device("cpu"))
+    assert plan.matches(params)
+    params[1].data = params[1].data.clone()                 # another address alone: looked up at every step
+    assert plan.matches(params)
+    state = {"layout": _layout(params[1])}
+    change(params[1])
+    assert not plan.matches(params)
+    if fits:
+        _check_layout(1, params[1], state)
+    else:
+        with pytest.raises(RuntimeError, match="parameter 1 is now"):
+            _check_layout(1, params[1], state)
+
+
+def test_a_module_converted_in_place():
+    from medical_image_segmentation_amd.utils.optim import _Plan8
+    m = torch.nn.Conv2d(4, 6, 3)
+    params = list(m.parameters())
+    plan = _Plan8(params, torch.device("cpu"))
+    m.bfloat16()
+    assert all(a is b for a, b in zip(params, m.parameters())) and not plan.matches(params)
+    m.float()
+    assert plan.matches(params)
+    m.to(memory_format=torch.channels_last)
+    assert not plan.matches(params)
+    m.half()
+    with pytest.raises(TypeError, match="float32 and bfloat16"):
+        _Plan8(params, torch.device("cpu"))
+
+
+def test_layouts_that_are_the_same_memory_order():
+    from medical_image_segmentation_amd.utils.optim import _layout
+    w = torch.zeros(8, 3, 1, 1)
+    assert _layout(w) == _layout(w.contiguous(memory_format=torch.channels_last)) == ((8, 3, 1, 1), (0, 1))
+    w = torch.zeros(8, 3, 2, 2)
+    assert _layout(w) != _layout(w.contiguous(memory_format=torch.channels_last))
+    assert _layout(torch.zeros(4, 0, 3)) == _layout(torch.zeros(3, 0, 4).transpose(0, 2)) == ((4, 0, 3), ())
+    assert _layout(torch.zeros(())) == ((), ())
+
+
+def test_gradients_of_another_size_are_not_taken():
+    """The kernels read as many elements of a gradient as its parameter has."""
+    from medical_image_segmentation_amd import functional as F_
+    from medical_image_segmentation_amd.utils.optim import _Plan8, _Table8
+    p, q = _params((4,), (7,))
+    p.grad, q.grad = torch.ones(4), torch.ones(7)
+    assert F_._native().step_pointers([p, q], -1) == [p.data_ptr(), p.grad.data_ptr(), q.data_ptr(), q.grad.data_ptr()]
+    q.data = torch.zeros(9)
+    assert q.grad.numel() == 7 and F_._native().step_pointers([p, q], -1) == []
+    plan = _Plan8([p, q], torch.device("cpu"))
+    plan.device = type("Host", (), {"index": -1})        # (what a host tensor gives for its device)
+    table = object.__new__(_Table8)
+    table.plan, table.order, table.plain, table.dtypes = plan, [p, q], [True, True], [torch.float32] * 2
+    with pytest.raises(RuntimeError, match="type, device and shape"):
+        table.addresses()

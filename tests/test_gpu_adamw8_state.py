@@ -1,0 +1,109 @@
+"""GPU suite: AdamW8 when parameters or its state change between two steps.  Codes and scales are compared with the update in
+64 bits; tolerances of the parameters as in test_gpu_adamw8.py."""
+import copy
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_adamw8 import DEV, HP, Oracle, _check, _grads, _pad, _params
+
+pytestmark = pytest.mark.gpu
+
+
+def _step(opt, params, o, k, dtype):
+    _grads(params, 200 + k)
+    o.p = np.concatenate([_pad(p) for p in params])
+    o.advance(params)
+    opt.step()
+    _check(opt, params, o, dtype, f"step {k}")
+
+
+def test_a_model_converted_between_steps():
+    """float32 -> bfloat16 -> float32 under one optimizer: the moments go on, every step is the formula's for the type that the
+    parameters have then."""
+    from medical_image_segmentation_amd.utils.optim import AdamW8
+    params = _params([1, 127, 129, 5000, 12289, 0], torch.float32, 31)
+    m = torch.nn.Module()
+    for i, p in enumerate(params):
+        m.register_parameter(f"p{i}", p)
+    opt, o = AdamW8(params, **HP), Oracle(params, HP)
+    _step(opt, params, o, 0, torch.float32)
+    m.bfloat16()
+    assert all(p is q for p, q in zip(params, m.parameters())) and params[3].dtype == torch.bfloat16
+    _step(opt, params, o, 1, torch.bfloat16)
+    _step(opt, params, o, 2, torch.bfloat16)
+    m.float()
+    _step(opt, params, o, 3, torch.float32)
+    for p in params:                                    # another address
+        p.data = p.data.clone()
+    _step(opt, params, o, 4, torch.float32)
+    assert [opt.state[p]["step"] for p in params] == [5] * 6
+
+
+def test_a_gradient_of_the_type_before():
+    from medical_image_segmentation_amd.utils.optim import AdamW8
+    p = _params([300], torch.float32, 32)[0]
+    opt = AdamW8([p], **HP)
+    _grads([p], 1)
+    opt.step()
+    p.data = p.data.bfloat16()                          # its gradient stays float32
+    before = p.detach().clone()
+    with pytest.raises(RuntimeError, match="type, device and shape"):
+        opt.step()
+    assert torch.equal(p, before) and opt.state[p]["step"] == 1
+
+
+@pytest.mark.parametrize("change", ["channels_last", "fewer", "more", "transposed"])
+def test_another_shape_or_memory_order_raises(change):
+    from medical_image_segmentation_amd.utils.optim import AdamW8, clip_and_step
+    torch.manual_seed(2)
+    p = torch.nn.Parameter(torch.randn(8, 6, 3, 3, device=DEV))
+    opt = AdamW8([p], **HP)
+    p.grad = torch.randn_like(p)
+    opt.step()
+    kept = p.data
+    p.data = {"channels_last": lambda t: t.contiguous(memory_format=torch.channels_last), "fewer": lambda t: t[:4].clone(),
+              "more": lambda t: torch.cat([t, t]), "transposed": lambda t: t.transpose(0, 1)}[change](p.data)
+    p.grad = None
+    p.grad = torch.zeros_like(p)
+    before, codes = p.detach().clone(), opt.state[p]["exp_avg"].clone()
+    for step in (opt.step, lambda: clip_and_step(opt, [p], 1.0), lambda: opt.moments(p)):
+        with pytest.raises(RuntimeError, match="parameter 0 is now"):
+            step()
+    assert torch.equal(p, before) and torch.equal(opt.state[p]["exp_avg"], codes) and opt.state[p]["step"] == 1
+    p.data, p.grad = kept, None                          # back again: it goes on
+    p.grad = torch.randn_like(p)
+    opt.step()
+    assert opt.state[p]["step"] == 2
+
+
+def _captured():
+    from medical_image_segmentation_amd.model.utils.modules import ChannelMLP
+    from medical_image_segmentation_amd.utils.graph_step import GraphedTrainStep
+    from medical_image_segmentation_amd.utils.optim import AdamW8
+    torch.manual_seed(6)
+    m = ChannelMLP(16, expansion=2, num_groups=4).to(DEV)
+    x = torch.randn(2, 16, 6, 6, device=DEV).contiguous(memory_format=torch.channels_last)
+    opt = AdamW8(m.parameters(), **HP)
+    step = GraphedTrainStep(m, opt, lambda m, x, y: ((m(x) - y).square().mean(), {}), x, torch.randn_like(x), max_norm=0.5)
+    step(x, x)
+    return m, opt, step, x
+
+
+@pytest.mark.parametrize("change", ["type", "address"])
+def test_a_captured_step_refuses_parameters_that_it_was_not_captured_for(change):
+    """The capture writes to the addresses that the parameters had: those may be another tensor's by now."""
+    m, opt, step, x = _captured()
+    taken = opt.state[m.narrow.weight]["step"]
+    kept = [p.data for p in m.parameters()]              # (alive, so that nothing is written to memory that was given back)
+    if change == "type":
+        m.bfloat16()
+    else:
+        m.narrow.weight.data = m.narrow.weight.data.clone()
+    with pytest.raises(RuntimeError, match="capture the step again"):
+        step(x, x)
+    for p, t in zip(m.parameters(), kept):
+        p.data = t
+    step(x, x)
+    assert opt.state[m.narrow.weight]["step"] == taken + 1
