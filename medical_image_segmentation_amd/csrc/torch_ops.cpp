@@ -10,6 +10,10 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/graph_task.h>
+
+#include <unordered_set>
+#include <vector>
 
 #include "../../include/misamd.h"
 
@@ -39,18 +43,37 @@ void check(int rc, const char* name) {
 
 // A backward pass under capture must not reach a leaf whose gradient node was made on the default stream, which cannot join
 // a capture: the node lives as long as any graph that uses the leaf, here one from before the capture.  (The engine would
-// wait on that stream at the end of the pass and the capture would end with the process.)
-void refuse_stale_leaf(const Tensor& t, bool capturing, const char* name) {
-  if (!capturing || !t.defined() || !t.requires_grad() || !t.is_leaf()) return;
-  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-  if (!node) return;
-  const auto made_on = node->stream();
-  TORCH_CHECK(!made_on || made_on->id() != c10::hip::getDefaultHIPStream(t.get_device()).id(), name,
-              ": an eager graph of the same leaf is alive; drop the tensors that hold it (outputs, losses) before capturing a "
-              "backward pass");
+// wait on that stream at the end of the pass and the capture would end with the process.)  Looked at are all leaves that this
+// pass will reach from the running node on, behind views, casts and other operations too; only under capture, so that
+// walking the graph costs an eager pass nothing.
+void refuse_stale_leaves(const char* name) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto running = torch::autograd::get_current_node();
+  if (!running) return;
+  const auto* wanted = torch::autograd::get_current_graph_task_exec_info();       // empty: all nodes are executed
+  std::vector<torch::autograd::Node*> todo{running.get()};
+  std::unordered_set<torch::autograd::Node*> seen;
+  while (!todo.empty()) {
+    torch::autograd::Node* node = todo.back();
+    todo.pop_back();
+    for (const auto& edge : node->next_edges()) {
+      torch::autograd::Node* next = edge.function.get();
+      if (!next || !seen.insert(next).second) continue;
+      if (wanted && !wanted->empty()) {
+        const auto found = wanted->find(next);
+        if (found == wanted->end() || !found->second.should_execute()) continue;
+      }
+      if (!next->next_edges().empty()) {
+        todo.push_back(next);
+        continue;
+      }
+      const auto made_on = next->stream();
+      TORCH_CHECK(!made_on || made_on->id() != c10::hip::getDefaultHIPStream(made_on->device_index()).id(), name,
+                  ": an eager graph of the same leaf is alive; drop the tensors that hold it (outputs, losses) before capturing "
+                  "a backward pass");
+    }
+  }
 }
-
-bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
 
 // Gradients that raise when they are differentiated with respect to what they were formed from: the backward is not
 // differentiable itself.
@@ -95,8 +118,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
     const bool twice = at::GradMode::is_enabled();         // create_graph=True
     at::NoGradGuard no_grad;
     c10::DeviceGuard guard(x.device());
-    const bool captured = capturing();
-    for (const Tensor& t : {x, w, b}) refuse_stale_leaf(t, captured, "group_norm_act");
+    refuse_stale_leaves("group_norm_act");
     const int64_t B = x.size(0), C = x.size(1), HW = x.size(2) * x.size(3);
     const bool some = x.numel() > 0;
     Tensor dx, dw, db;
@@ -155,8 +177,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     const bool twice = at::GradMode::is_enabled();         // create_graph=True
     at::NoGradGuard no_grad;
     c10::DeviceGuard guard(x.device());
-    const bool captured = capturing();
-    for (const Tensor& t : {x, w, b}) refuse_stale_leaf(t, captured, "linear_act");
+    refuse_stale_leaves("linear_act");
     const int64_t N = w.size(0), K = w.size(1), M = x.numel() / K;
     Tensor dx, dw, db, dr;
     Wanted wanted{ctx};
