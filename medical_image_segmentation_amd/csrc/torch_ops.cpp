@@ -235,6 +235,24 @@ class Layouts {
   std::vector<One> kept_;
 };
 
+// Whether the values of an optimizer's `state` are still these dicts, in this order, and hold these tensors (as many to a dict
+// as there are keys; None: no such entry): a user may clear the state, or put other dicts or tensors in its place.
+bool state_holds(const pybind11::dict& state, const pybind11::list& dicts, const pybind11::tuple& keys,
+                 const pybind11::list& tensors) {
+  const Py_ssize_t n = PyList_GET_SIZE(dicts.ptr()), k = PyTuple_GET_SIZE(keys.ptr());
+  if (PyDict_Size(state.ptr()) != n || PyList_GET_SIZE(tensors.ptr()) != n * k) return false;
+  PyObject *key, *value;
+  Py_ssize_t at = 0;
+  for (Py_ssize_t i = 0; PyDict_Next(state.ptr(), &at, &key, &value); i++) {
+    if (value != PyList_GET_ITEM(dicts.ptr(), i) || !PyDict_Check(value)) return false;
+    for (Py_ssize_t j = 0; j < k; j++) {
+      PyObject* held = PyDict_GetItem(value, PyTuple_GET_ITEM(keys.ptr(), j));
+      if ((held ? held : Py_None) != PyList_GET_ITEM(tensors.ptr(), i * k + j)) return false;
+    }
+  }
+  return true;
+}
+
 // The pointers [parameter, gradient, parameter, ...] of parameters whose gradients lie in the same memory order, type and
 // device; empty if one does not (the caller then looks at them one by one).
 std::vector<int64_t> step_pointers(const std::vector<Tensor>& params, int64_t device) {
@@ -257,5 +275,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("group_norm_act", &group_norm_act, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("linear_act", &linear_act, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("step_pointers", &step_pointers);
+  m.def("state_holds", &state_holds);
   pybind11::class_<Layouts>(m, "Layouts").def(pybind11::init<std::vector<Tensor>>()).def("hold", &Layouts::hold);
 }

@@ -129,13 +129,15 @@ def clip_and_step(optimizer, params, max_norm=1.0):
     params = [p for p in params]
     F_.flush_wgrad_reduces()       # (a no-op after a finished backward pass)
     if isinstance(optimizer, AdamW8):
-        stepped, given = optimizer._stepped(), [p for p in params if p.grad is not None]
-        same = len(stepped) == len(given) and all(map(operator.is_, stepped, given))
-        if not same and (len(stepped) != len(given) or {id(p) for p in given} != {id(p) for p in stepped}):
-            norm = torch.nn.utils.clip_grad_norm_(params, max_norm=max_norm)   # a norm over other tensors than are stepped
-            optimizer.step()
-            return norm
-        return optimizer._launch(float(max_norm), stepped)
+        held = optimizer._params()
+        stepped = [p for p in held if p.grad is not None]
+        if len(params) != len(held) or not all(map(operator.is_, params, held)):
+            given = [p for p in params if p.grad is not None]
+            if len(stepped) != len(given) or {id(p) for p in given} != {id(p) for p in stepped}:
+                norm = torch.nn.utils.clip_grad_norm_(params, max_norm=max_norm)   # a norm over other tensors than are stepped
+                optimizer.step()
+                return norm
+        return optimizer._launch(float(max_norm), stepped, held)
     fast = _fast_path(optimizer, params)
     if fast is not None:
         return _launch(optimizer, fast, max_norm)
@@ -272,6 +274,20 @@ def _check_layout(i, p, s):
                            "back, or delete the parameter's state to begin again")
 
 
+def _check_codes(i, n, s):
+    """Whether state `s` of parameter `i` (n elements) holds moments; raises where it holds something else."""
+    held = [k for k in AdamW8._STATE if k in s]
+    if not held:
+        return False
+    for k in AdamW8._STATE:
+        if k not in s:
+            raise ValueError(f"not an AdamW8 state: parameter {i} has no {k}")
+        want = _blocks(n) * (1 if k.endswith("_scale") else BLOCK8)
+        if s[k].dtype != torch.uint8 or s[k].numel() != want:
+            raise ValueError(f"parameter {i}: {k} should be {want} bytes, got {s[k].numel()} of {s[k].dtype}")
+    return True
+
+
 class AdamW8(torch.optim.Optimizer):
     """AdamW with both moments in 8 bits, one launch for all tensors (two when the gradient norm is clipped).
 
@@ -285,8 +301,9 @@ class AdamW8(torch.optim.Optimizer):
                 "exp_avg_scale", "exp_avg_sq_scale": uint8, one per 128,
                 "layout": (shape, dimensions by falling stride)}; `moments(p)` gives their float32 values.
     The codes follow the elements' order in memory.  A parameter may change its type, device or address between steps
-    (Module.bfloat16(), .data = ...), but not its shape or memory order: the step raises then.  A parameter without a
-    gradient is left alone, as in torch.
+    (Module.bfloat16(), .data = ...), but not its shape or memory order: the step raises then.  A cleared state begins again
+    at step 1 with moments of zero, one put in its place is gone on from.  A parameter without a gradient is left alone, as
+    in torch.
     """
     _STATE = ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale")
     _plan = None
@@ -318,17 +335,13 @@ class AdamW8(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         n = {i: p.numel() for i, p in enumerate(q for g in self.param_groups for q in g["params"])}
         for i, s in state_dict["state"].items():
-            for k in self._STATE:
-                if k not in s:
-                    raise ValueError(f"not an AdamW8 state: parameter {i} has no {k}")
-                want = _blocks(n[i]) * (1 if k.endswith("_scale") else BLOCK8) if i in n else None
-                if want is not None and (s[k].dtype != torch.uint8 or s[k].numel() != want):
-                    raise ValueError(f"parameter {i}: {k} should be {want} bytes, got {s[k].numel()} of {s[k].dtype}")
+            if i in n and not _check_codes(i, n[i], s):
+                raise ValueError(f"not an AdamW8 state: parameter {i} has no {self._STATE[0]}")
         # (the codes go past torch's loading, which would take them through the parameters' floating-point type)
         states = state_dict["state"]
         rest = {i: {k: v for k, v in s.items() if k not in self._STATE} for i, s in states.items()}
         super().load_state_dict({**state_dict, "state": rest})
-        params = [p for g in self.param_groups for p in g["params"]]
+        params = self._params()
         for i, p in zip((i for g in state_dict["param_groups"] for i in g["params"]), params):
             if i in states:
                 self.state[p].update({k: states[i][k].reshape(-1) for k in self._STATE}, step=int(states[i]["step"]))
@@ -339,20 +352,23 @@ class AdamW8(torch.optim.Optimizer):
             for s in self.state.values():
                 s.update({k: s[k].clone() for k in self._STATE if k in s})
 
-    def _stepped(self):
-        return [p for g in self.param_groups for p in g["params"] if p.grad is not None]
+    def _params(self):
+        return [p for g in self.param_groups for p in g["params"]]
 
-    def _flat(self):
-        """The flat moment buffers, laid out over all parameters; state[p] holds views of them."""
-        params = [p for g in self.param_groups for p in g["params"]]
+    def _flat(self, params=None):
+        """The flat moment buffers, laid out over all parameters (`params`, where the caller has their list); state[p] holds
+        views of them."""
+        params = params or self._params()
         plan = self._plan
-        if plan is not None and plan.matches(params):
+        if plan is not None and plan.matches(params) and plan.holds(self.state):
             return plan
         devs = {p.device for p in params}
         if len(devs) != 1 or next(iter(devs)).type != "cuda":
             raise RuntimeError(f"AdamW8 needs all parameters on one GPU, got {sorted(map(str, devs))}")
         for i, p in enumerate(params):
-            _check_layout(i, p, self.state.get(p, {}))
+            s = self.state.get(p, {})
+            _check_layout(i, p, s)
+            _check_codes(i, p.numel(), s)
         plan = self._plan = _Plan8(params, next(iter(devs)))
         views = [buf.split([(b1 - b0) * w for b0, b1 in plan.spans] + [buf.numel() - plan.blocks * w])
                  for buf, w in zip(plan.buffers, (BLOCK8, 1, BLOCK8, 1))]
@@ -363,12 +379,13 @@ class AdamW8(torch.optim.Optimizer):
                 if k in s:                        # (codes behind the last element stay zero)
                     n = p.numel() if v is views[0] or v is views[2] else v[i].numel()
                     to.append(v[i][:n])
-                    given.append(s[k][:n])
+                    given.append(s[k].reshape(-1)[:n])
                 s[k] = v[i]
             s["step"] = int(s.get("step", 0))
             s["layout"] = _layout(p)
         if to:
             torch._foreach_copy_(to, given)
+        plan.keep(self.state)
         return plan
 
     def moments(self, p=None):
@@ -393,18 +410,19 @@ class AdamW8(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        self._launch(None, self._stepped())
+        held = self._params()
+        self._launch(None, [p for p in held if p.grad is not None], held)
         return loss
 
-    def _launch(self, max_norm, params):
-        """One step of `params`, those with a gradient; max_norm None: no norm is formed.  Returns the total gradient norm
-        otherwise."""
+    def _launch(self, max_norm, params, held):
+        """One step of `params`, those with a gradient of all that are `held`; max_norm None: no norm is formed.  Returns the
+        total gradient norm otherwise."""
         if not params:
             return torch.zeros(()) if max_norm is not None else None
         if params[0].is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("an AdamW8 step cannot be captured as it is (its step number would be frozen): use "
                                "CapturedStep or GraphedTrainStep")
-        table = self._flat().table(self.param_groups, self.state, params)
+        table = self._flat(held).table(self.param_groups, self.state, params)
         norm = table.launch(max_norm)
         for states in table.states:
             k = states[0]["step"] + 1
@@ -436,6 +454,14 @@ class _Plan8:
     def matches(self, params):
         """Whether these are the parameters that buffers and tables were made for, in type, device, shape and strides too."""
         return len(params) == len(self.params) and all(map(operator.is_, params, self.params)) and self.layouts.hold()
+
+    def keep(self, state):
+        """Takes note of the state that the buffers serve: `holds` says whether it is still that one."""
+        self.states = list(state.values())
+        self.held = [s.get(k) for s in self.states for k in AdamW8._STATE]
+
+    def holds(self, state):
+        return F_._native().state_holds(state, self.states, AdamW8._STATE, self.held)
 
     def table(self, groups, state, params):
         """The launch tables for `params`, the parameters that have a gradient now."""
@@ -554,7 +580,8 @@ class _CapturedStep8:
     RING, WIDTH = 8, 32           # bytes per run's constants (20 used)
 
     def __init__(self, optimizer, params, max_norm):
-        self.optimizer, self.params, self.max_norm = optimizer, optimizer._stepped(), float(max_norm)
+        self.optimizer, self.max_norm = optimizer, float(max_norm)
+        self.params = [p for p in optimizer._params() if p.grad is not None]
         if {id(p) for p in params if p.grad is not None} != {id(p) for p in self.params} or not self.params:
             raise RuntimeError("CapturedStep needs the gradients of exactly the tensors that the optimizer steps")
         if any(optimizer.state[p].get("step", 0) < 1 for p in self.params):
@@ -574,8 +601,8 @@ class _CapturedStep8:
         self.norm = None
 
     def prepare(self):
-        if self.optimizer._plan is not self.plan:
-            raise RuntimeError("the optimizer's state was replaced after the capture")
+        if self.optimizer._plan is not self.plan or not self.plan.holds(self.optimizer.state):
+            raise RuntimeError("the optimizer's state was replaced after the capture: capture the step again")
         if not self.plan.matches(self.plan.params) or [p.data_ptr() for p in self.table.order] != self.addresses:
             raise RuntimeError("a parameter was converted or its memory replaced after the capture: capture the step again")
         if not self.table.serves(self.params):
