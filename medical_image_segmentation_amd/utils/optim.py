@@ -267,11 +267,14 @@ def _layout(p):
 
 
 def _check_layout(i, p, s):
-    """The codes of state `s` follow the memory of the tensor they were made for: they mean nothing in another order."""
-    if "layout" in s and s["layout"] != _layout(p):
-        raise RuntimeError(f"AdamW8: parameter {i} is now {tuple(p.shape)} with strides {p.stride()}, its moments were made for "
-                           f"shape {s['layout'][0]} with the dimensions {s['layout'][1]} by falling stride: convert the model "
-                           "back, or delete the parameter's state to begin again")
+    """The codes of state `s` follow the memory of the tensor they were made for: they mean nothing in another order.  Without a
+    record of it they are taken for row-major."""
+    shape, order = _layout(p)
+    made = s.get("layout", (shape, sorted(order)))
+    if (tuple(made[0]), tuple(made[1])) != (shape, order):
+        raise RuntimeError(f"AdamW8: parameter {i} is now {shape} with strides {p.stride()}, its moments were made for shape "
+                           f"{tuple(made[0])} with the dimensions {tuple(made[1])} by falling stride: convert the model back, or "
+                           "delete the parameter's state to begin again")
 
 
 def _check_codes(i, n, s):
@@ -333,18 +336,23 @@ class AdamW8(torch.optim.Optimizer):
         self._plan = None
 
     def load_state_dict(self, state_dict):
-        n = {i: p.numel() for i, p in enumerate(q for g in self.param_groups for q in g["params"])}
-        for i, s in state_dict["state"].items():
-            if i in n and not _check_codes(i, n[i], s):
-                raise ValueError(f"not an AdamW8 state: parameter {i} has no {self._STATE[0]}")
+        names = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(names, self._params()):        # (before anything is replaced; torch checks the groups' lengths)
+            s = state_dict["state"].get(i)
+            if s is not None:
+                if not _check_codes(i, p.numel(), s):
+                    raise ValueError(f"not an AdamW8 state: parameter {i} has no {self._STATE[0]}")
+                _check_layout(i, p, s)
         # (the codes go past torch's loading, which would take them through the parameters' floating-point type)
         states = state_dict["state"]
-        rest = {i: {k: v for k, v in s.items() if k not in self._STATE} for i, s in states.items()}
+        past = self._STATE + ("layout",)
+        rest = {i: {k: v for k, v in s.items() if k not in past} for i, s in states.items()}
         super().load_state_dict({**state_dict, "state": rest})
         params = self._params()
-        for i, p in zip((i for g in state_dict["param_groups"] for i in g["params"]), params):
+        for i, p in zip(names, params):
             if i in states:
-                self.state[p].update({k: states[i][k].reshape(-1) for k in self._STATE}, step=int(states[i]["step"]))
+                self.state[p].update({k: states[i][k].reshape(-1) for k in self._STATE}, step=int(states[i]["step"]),
+                                     layout=_layout(p))
         self._plan = None
         if all(p.is_cuda for p in params) and len({p.device for p in params}) == 1:
             self._flat()
@@ -366,9 +374,9 @@ class AdamW8(torch.optim.Optimizer):
         if len(devs) != 1 or next(iter(devs)).type != "cuda":
             raise RuntimeError(f"AdamW8 needs all parameters on one GPU, got {sorted(map(str, devs))}")
         for i, p in enumerate(params):
-            s = self.state.get(p, {})
-            _check_layout(i, p, s)
-            _check_codes(i, p.numel(), s)
+            if self.state.get(p):
+                _check_layout(i, p, self.state[p])
+                _check_codes(i, p.numel(), self.state[p])
         plan = self._plan = _Plan8(params, next(iter(devs)))
         views = [buf.split([(b1 - b0) * w for b0, b1 in plan.spans] + [buf.numel() - plan.blocks * w])
                  for buf, w in zip(plan.buffers, (BLOCK8, 1, BLOCK8, 1))]

@@ -129,3 +129,60 @@ def test_what_is_put_into_the_state_is_checked():
             _check_codes(0, 300, {**good, k: good[k].float()})
         with pytest.raises(ValueError, match="bytes, got"):
             _check_codes(0, 300, {**good, k: good[k][:-1]})
+
+
+def _saved(p, step=3):
+    """A state dict of AdamW8 for one parameter, as a run that held it in this memory order leaves it."""
+    from medical_image_segmentation_amd.utils.optim import AdamW8, _layout
+    opt, n = AdamW8([p]), -(-p.numel() // 128)
+    codes = lambda k, seed: torch.randint(0, 255, (k,), generator=torch.Generator().manual_seed(seed), dtype=torch.uint8)  # noqa: E731
+    opt.state[p] = dict(step=step, exp_avg=codes(128 * n, 1), exp_avg_scale=codes(n, 2), exp_avg_sq=codes(128 * n, 3),
+                        exp_avg_sq_scale=codes(n, 4), layout=_layout(p))
+    return opt.state_dict()
+
+
+def test_a_checkpoint_is_loaded_into_its_own_memory_order_alone():
+    """The codes lie in the order of the parameter's memory: in another one every moment would be another element's."""
+    import io
+    from medical_image_segmentation_amd.utils.optim import AdamW8
+    torch.manual_seed(0)
+    rows = torch.randn(6, 4, 3, 3)
+    last = rows.contiguous(memory_format=torch.channels_last)
+    for made in (rows, last):
+        file = io.BytesIO()
+        torch.save(_saved(torch.nn.Parameter(made.clone(memory_format=torch.preserve_format))), file)
+        file.seek(0)
+        state = torch.load(file, weights_only=True)
+        for to in (rows, last):
+            p = torch.nn.Parameter(to.clone(memory_format=torch.preserve_format))
+            opt = AdamW8([p], lr=0.5)
+            if made is to:
+                opt.load_state_dict(state)
+                assert torch.equal(opt.state[p]["exp_avg"], state["state"][0]["exp_avg"]) and opt.state[p]["step"] == 3
+                assert opt.param_groups[0]["lr"] == 1e-3
+            else:
+                with pytest.raises(RuntimeError, match="parameter 0 is now"):
+                    opt.load_state_dict(state)
+                assert not opt.state and opt.param_groups[0]["lr"] == 0.5         # nothing was replaced
+        del state["state"][0]["layout"]                          # no record: row-major
+        opt = AdamW8([torch.nn.Parameter(rows.clone())])
+        opt.load_state_dict(state)
+        opt = AdamW8([torch.nn.Parameter(last.clone(memory_format=torch.preserve_format))])
+        with pytest.raises(RuntimeError, match="by falling stride"):
+            opt.load_state_dict(state)
+    with pytest.raises(RuntimeError, match="parameter 0 is now"):
+        AdamW8([torch.nn.Parameter(rows.reshape(4, 6, 3, 3))]).load_state_dict(_saved(torch.nn.Parameter(rows)))
+
+
+def test_a_state_dict_may_number_its_parameters_otherwise():
+    from medical_image_segmentation_amd.utils.optim import AdamW8
+    p, q = _params((5,), (300,))
+    opt = AdamW8([p, q])
+    a, b = _saved(torch.nn.Parameter(p.detach().clone()), 4), _saved(torch.nn.Parameter(q.detach().clone()), 9)
+    groups = opt.state_dict()["param_groups"]
+    state = {"state": {7: a["state"][0], 3: b["state"][0]}, "param_groups": [{**groups[0], "params": [7, 3]}]}
+    opt.load_state_dict(state)
+    assert (opt.state[p]["step"], opt.state[q]["step"]) == (4, 9) and opt.state[q]["exp_avg"].numel() == 384
+    state["param_groups"][0]["params"] = [3, 7]
+    with pytest.raises(ValueError, match="parameter 3: exp_avg should be 128 bytes"):
+        opt.load_state_dict(state)

@@ -161,3 +161,28 @@ def test_a_captured_step_refuses_a_state_that_it_was_not_captured_for():
     opt.state.clear()
     with pytest.raises(RuntimeError, match="state was replaced after the capture"):
         step(x, x)
+
+
+def test_a_checkpoint_of_a_channels_last_model():
+    """Saved and loaded in its own order it goes on bit for bit; the same model in rows refuses it."""
+    from medical_image_segmentation_amd.utils.optim import AdamW8
+    torch.manual_seed(8)
+    w = torch.randn(8, 6, 3, 3, device=DEV)
+    last = w.contiguous(memory_format=torch.channels_last)
+    g = [torch.randn_like(w) for _ in range(3)]
+    a, b, c = (torch.nn.Parameter(t.clone(memory_format=torch.preserve_format)) for t in (last, last, w))
+    oa, ob, oc = (AdamW8([p], **HP) for p in (a, b, c))
+    for t in g[:2]:
+        a.grad = t.contiguous(memory_format=torch.channels_last)
+        oa.step()
+    saved = copy.deepcopy(oa.state_dict())
+    ob.load_state_dict(saved)
+    with torch.no_grad():
+        b.copy_(a)
+    a.grad, b.grad = g[2].contiguous(memory_format=torch.channels_last), g[2]
+    oa.step()
+    ob.step()
+    assert torch.equal(a, b) and all(torch.equal(x, y) for x, y in zip(oa.moments(a), ob.moments(b)))
+    with pytest.raises(RuntimeError, match="parameter 0 is now"):
+        oc.load_state_dict(saved)
+    assert not oc.state
