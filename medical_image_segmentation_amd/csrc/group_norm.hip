@@ -9,8 +9,9 @@
 // A workgroup owns a range of pixels and a slab of at most 256 channel vectors that starts and ends with a group
 // (or lies inside one group, when a group is wider); a thread keeps one channel vector and walks the pixels, so a
 // wave reads contiguous memory and everything that belongs to a channel stays in registers.
-// The statistics are plain sums of x and x*x in 64 bits: on this chip a double add costs what a float add costs,
-// and 53 bits make the subtraction E[x^2] - mean^2 harmless (any spread that the input's 24 bits can hold survives).
+// The statistics are sums of d = x - K and d*d in 64 bits, K the group's first value: mean = K + E[d], var = E[d^2] - E[d]^2.
+// K is as near to the mean as the group's values are, so the subtraction is harmless at any mean: a spread of one unit in the
+// last place of float32 survives.  On this chip a double add costs what a float add costs.
 // Sums over pixels are combined in a fixed order: results repeat bit for bit.
 #include <algorithm>
 
@@ -68,7 +69,27 @@ __device__ __forceinline__ Slab slab_of(const Shape& s, int i) {
   return r;
 }
 
-// sums[b][chunk*parts + part][g] = (sum x, sum x*x) over the chunk's pixels and the slab's channels of g.
+// f(i, group of channel c + i, whether that is another group than channel c + i - 1's) for i < V, with one division.
+template <int V, typename F> __device__ __forceinline__ void with_groups(int c, int Cg, F&& f) {
+  int g = c / Cg, left = Cg - (c - g * Cg);
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    const bool other = i > 0 && left == 0;
+    if (other) {
+      g++;
+      left = Cg;
+    }
+    f(i, g, i == 0 || other);
+    left--;
+  }
+}
+
+// K of group g.  (Where it is not finite the statistics would not be either.)
+template <typename T> __device__ __forceinline__ double first_of(const T* __restrict__ sample, int g, int Cg) {
+  return (double)to_f32(sample[(int64_t)g * Cg]);
+}
+
+// sums[b][chunk*parts + part][g] = (sum d, sum d*d) over the chunk's pixels and the slab's channels of g.
 // U: channels of a vector that are sure to share a group (a power of two that divides V and the group), so a thread holds
 // V/U pairs of sums and not V: few enough registers for eight waves to a SIMD, which the stream of loads needs.
 // Bound by HBM: 16x32x512^2 bf16 (268 MB) in 72 us behind a kernel whose output is still being written back, 3.7 TB/s; its
@@ -84,14 +105,19 @@ __global__ __launch_bounds__(GN_THREADS) void gn_sums_kernel(const T* __restrict
   const int64_t p0 = (int64_t)blockIdx.x * s.ppc, p1 = min(p0 + s.ppc, s.HW);
   const bool on = pr < s.PR && cv * V < sl.nc;
   if (on) {
-    double a1[N], a2[N];
-#pragma unroll
-    for (int k = 0; k < N; k++) a1[k] = a2[k] = 0.0;
-    const T* xp = x + (int64_t)b * s.HW * s.C + sl.c0 + cv * V;
+    double a1[N], a2[N], first[N];
+    const T* sample = x + (int64_t)b * s.HW * s.C;
+    double of_group = 0.0;
+    with_groups<N>((sl.c0 + cv * V) / U, s.Cg / U, [&](int k, int g, bool other) {
+      if (other) of_group = first_of(sample, g, s.Cg);
+      first[k] = of_group;
+      a1[k] = a2[k] = 0.0;
+    });
+    const T* xp = sample + sl.c0 + cv * V;
     auto add = [&](const Vec<T, V>& v) {
 #pragma unroll
       for (int k = 0; k < V; k++) {
-        const double d = (double)to_f32(v.t[k]);
+        const double d = (double)to_f32(v.t[k]) - first[k / U];
         a1[k / U] += d;
         a2[k / U] = fma(d, d, a2[k / U]);
       }
@@ -159,16 +185,17 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
 }
 
-__device__ __forceinline__ double2 stats_of(double s1, double s2, double count, double eps) {
+__device__ __forceinline__ double2 stats_of(double s1, double s2, double first, double count, double eps) {
   const double mean = s1 / count;
   double var = s2 / count - mean * mean;
   if (var < 0.0) var = 0.0;                              // (NaN stays NaN)
-  return make_double2(mean, 1.0 / sqrt(var + eps));
+  return make_double2(first + mean, 1.0 / sqrt(var + eps));
 }
 
 // stats[b][g] = (mean, 1/sqrt(var + eps)); one wave per (b, g); a launch's latency, 3-5 us
-__global__ __launch_bounds__(64) void gn_stats_kernel(const double2* __restrict__ sums, int rows, int G, double count,
-                                                      double eps, double2* __restrict__ stats) {
+template <typename T>
+__global__ __launch_bounds__(64) void gn_stats_kernel(const T* __restrict__ x, Shape s, const double2* __restrict__ sums, int rows,
+                                                      int G, double count, double eps, double2* __restrict__ stats) {
   const int g = blockIdx.x, b = blockIdx.y, lane = threadIdx.x;
   double t1 = 0.0, t2 = 0.0;
   for (int r = lane; r < rows; r += 64) {
@@ -178,36 +205,27 @@ __global__ __launch_bounds__(64) void gn_stats_kernel(const double2* __restrict_
   }
   t1 = wave_sum64(t1);
   t2 = wave_sum64(t2);
-  if (lane == 0) stats[(int64_t)b * G + g] = stats_of(t1, t2, count, eps);
+  if (lane == 0) stats[(int64_t)b * G + g] = stats_of(t1, t2, first_of(x + (int64_t)b * s.HW * s.C, g, s.Cg), count, eps);
 }
 
-// What a thread holds of its V channels: u = (x - mean) * a + beta, a = rstd * gamma.
+// The mean in two floats: hi + lo.  One float would put x - mean off by up to 2^-25 |mean|, which is all of a spread that is
+// far smaller than the mean.
+__device__ __forceinline__ float mean_lo(double mean) { return (float)(mean - (double)(float)mean); }
+
+// What a thread holds of its V channels: u = (x - mean) * a + beta, a = rstd * gamma; mean is hi, and lo is in beta.
 template <int V> struct Consts {
   float mean[V], a[V], beta[V];
 };
-
-// f(i, group of channel c + i, whether that is another group than channel c + i - 1's) for i < V, with one division.
-template <int V, typename F> __device__ __forceinline__ void with_groups(int c, int Cg, F&& f) {
-  int g = c / Cg, left = Cg - (c - g * Cg);
-#pragma unroll
-  for (int i = 0; i < V; i++) {
-    const bool other = i > 0 && left == 0;
-    if (other) {
-      g++;
-      left = Cg;
-    }
-    f(i, g, i == 0 || other);
-    left--;
-  }
-}
 
 template <int V>
 __device__ __forceinline__ void load_consts(Consts<V>& k, const double2* __restrict__ stats, const float* __restrict__ gamma,
                                             const float* __restrict__ beta, int c, int Cg) {
   double2 st = make_double2(0.0, 0.0);
+  float lo[V];
   with_groups<V>(c, Cg, [&](int i, int g, bool other) {
     if (other) st = stats[g];
     k.mean[i] = (float)st.x;
+    lo[i] = mean_lo(st.x);
     k.a[i] = (float)st.y;
   });
 #pragma unroll
@@ -216,6 +234,8 @@ __device__ __forceinline__ void load_consts(Consts<V>& k, const double2* __restr
 #pragma unroll
     for (int i = 0; i < V; i++) k.a[i] *= gamma[c + i];
   }
+#pragma unroll
+  for (int i = 0; i < V; i++) k.beta[i] = fmaf(-lo[i], k.a[i], k.beta[i]);
 }
 
 // y from x: 2 passes over memory, 16x32x512^2 bf16 (537 MB) in 88 us, 6.1 TB/s.
@@ -244,7 +264,8 @@ __global__ __launch_bounds__(GN_THREADS) void gn_apply_kernel(const T* __restric
         t1 += v.x;
         t2 += v.y;
       }
-      const double2 st = stats_of(wave_sum64(t1), wave_sum64(t2), count, eps);
+      const double2 st = stats_of(wave_sum64(t1), wave_sum64(t2), first_of(x + (int64_t)b * s.HW * s.C, sl.g0 + g, s.Cg), count,
+                                  eps);
       if (lane == 0) {
         own[g] = st;
         if (blockIdx.x == 0) stats[sl.g0 + g] = st;      // (the parts of one group write the same)
@@ -272,7 +293,8 @@ __global__ __launch_bounds__(GN_THREADS) void gn_apply_kernel(const T* __restric
 // value in a million), its sign is taken from the 64-bit statistics, so that the mask is the definition's.
 template <int ACT>
 __device__ __forceinline__ float du_of(float x, float dy, float mean, float a, float beta, int c, int Cg,
-                                       const double2* __restrict__ stats, const float* __restrict__ gamma) {
+                                       const double2* __restrict__ stats, const float* __restrict__ gammas,
+                                       const float* __restrict__ betas) {
   const float u = fmaf(x - mean, a, beta);
   if constexpr (ACT == MIS_ACT_NONE) {
     return dy;
@@ -280,7 +302,7 @@ __device__ __forceinline__ float du_of(float x, float dy, float mean, float a, f
     bool pos = u > 0.f;
     if (fabsf(u) < 1e-6f * fmaf(fabsf(x) + fabsf(mean), fabsf(a), fabsf(beta))) {
       const double2 st = stats[c / Cg];
-      pos = ((double)x - st.x) * st.y * (gamma ? (double)gamma[c] : 1.0) + (double)beta > 0.0;
+      pos = ((double)x - st.x) * st.y * (gammas ? (double)gammas[c] : 1.0) + (betas ? (double)betas[c] : 0.0) > 0.0;
     }
     return pos ? dy : 0.f;
   } else {
@@ -319,15 +341,18 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_sums_kernel(const T* __rest
 #pragma unroll
       for (int i = 0; i < V; i++) {
         const float xf = to_f32(vx.t[i]);
-        const float du = du_of<ACT>(xf, to_f32(vd.t[i]), k.mean[i], k.a[i], k.beta[i], c + i, s.Cg, stats, gamma);
+        const float du = du_of<ACT>(xf, to_f32(vd.t[i]), k.mean[i], k.a[i], k.beta[i], c + i, s.Cg, stats, gamma, beta);
         a1[i] += du;
-        a2[i] = fmaf(du, xf - k.mean[i], a2[i]);         // times rstd at the end
+        a2[i] = fmaf(du, xf - k.mean[i], a2[i]);         // less lo a1, times rstd at the end
       }
     }
-    float rstd = 0.f;
+    float rstd = 0.f, lo = 0.f;
     with_groups<V>(c, s.Cg, [&](int i, int g, bool other) {
-      if (other) rstd = (float)stats[g].y;
-      red[(pr * s.CV + cv) * V + i] = make_float2(a1[i], a2[i] * rstd);
+      if (other) {
+        rstd = (float)stats[g].y;
+        lo = mean_lo(stats[g].x);
+      }
+      red[(pr * s.CV + cv) * V + i] = make_float2(a1[i], fmaf(-lo, a1[i], a2[i]) * rstd);
     });
   }
   __syncthreads();
@@ -443,16 +468,17 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_dx_kernel(const T* __restri
   const int c = sl.c0 + cv * V;
   Consts<V> k;
   load_consts<V>(k, stats, gamma, beta, c, s.Cg);
-  float q1[V], q2[V];                                    // dx = du a - q1 - (x - mean) q2
-  float rstd = 0.f;
+  float q1[V], q2[V];                                    // dx = du a - q1 - (x - hi) q2
+  float rstd = 0.f, lo = 0.f;
   float2 m = make_float2(0.f, 0.f);
   with_groups<V>(c, s.Cg, [&](int i, int g, bool other) {
     if (other) {
       rstd = (float)stats[g].y;
+      lo = mean_lo(stats[g].x);
       m = coef[(int64_t)b * s.G + g];
     }
-    q1[i] = rstd * m.x;
     q2[i] = rstd * rstd * m.y;
+    q1[i] = fmaf(-lo, q2[i], rstd * m.x);
   });
   const int64_t p0 = (int64_t)blockIdx.x * s.ppc, p1 = min(p0 + s.ppc, s.HW);
   const int64_t base = (int64_t)b * s.HW * s.C + c;
@@ -464,7 +490,7 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_dx_kernel(const T* __restri
 #pragma unroll
     for (int i = 0; i < V; i++) {
       const float xf = to_f32(vx.t[i]);
-      const float du = du_of<ACT>(xf, to_f32(vd.t[i]), k.mean[i], k.a[i], k.beta[i], c + i, s.Cg, stats, gamma);
+      const float du = du_of<ACT>(xf, to_f32(vd.t[i]), k.mean[i], k.a[i], k.beta[i], c + i, s.Cg, stats, gamma, beta);
       vd.t[i] = from_f32<T>(fmaf(du, k.a[i], -fmaf(xf - k.mean[i], q2[i], q1[i])));
     }
     *(typename Bits<T, V>::type*)(dx + base + p * s.C) = vd.u;
@@ -529,6 +555,8 @@ __global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_kernel(const T* __
     const int p = min(pr + i * s.PR, HW - 1);
     v[i].u = *(const typename Bits<T, V>::type*)(x + base + (int64_t)p * s.C);
   }
+  const T* sample = x + (int64_t)b * s.HW * s.C;
+  const double first = first_of(sample, (sl.c0 + (on ? cv * V : 0)) / s.Cg, s.Cg);
   double s1 = 0.0, s2 = 0.0;
   if (on) {
 #pragma unroll
@@ -536,7 +564,7 @@ __global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_kernel(const T* __
       if (pr + i * s.PR < HW) {
 #pragma unroll
         for (int k = 0; k < V; k++) {
-          const double d = (double)to_f32(v[i].t[k]);
+          const double d = (double)to_f32(v[i].t[k]) - first;
           s1 += d;
           s2 = fma(d, d, s2);
         }
@@ -547,7 +575,7 @@ __global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_kernel(const T* __
   group_sums(s1, s2, s.CV, GV, sl.ng, s.PR, red, grp);
   const double count = (double)s.HW * s.Cg;
   if (tid < sl.ng) {
-    const double2 st = stats_of(grp[tid].x, grp[tid].y, count, eps);
+    const double2 st = stats_of(grp[tid].x, grp[tid].y, first_of(sample, sl.g0 + tid, s.Cg), count, eps);
     grp[tid] = st;
     stats[(int64_t)b * s.G + sl.g0 + tid] = st;
   }
@@ -594,7 +622,8 @@ __global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_bwd_kernel(const T
   }
   Consts<V> k;
   load_consts<V>(k, stats, gamma, beta, c, s.Cg);
-  const float rstd = (float)stats[c / s.Cg].y;
+  const double2 st = stats[c / s.Cg];
+  const float rstd = (float)st.y, lo = mean_lo(st.x);
   float a1[V], a2[V];
 #pragma unroll
   for (int j = 0; j < V; j++) a1[j] = a2[j] = 0.f;
@@ -605,7 +634,7 @@ __global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_bwd_kernel(const T
 #pragma unroll
         for (int j = 0; j < V; j++) {
           const float xf = to_f32(vx[i].t[j]);
-          const float du = du_of<ACT>(xf, to_f32(vd[i].t[j]), k.mean[j], k.a[j], k.beta[j], c + j, s.Cg, stats, gamma);
+          const float du = du_of<ACT>(xf, to_f32(vd[i].t[j]), k.mean[j], k.a[j], k.beta[j], c + j, s.Cg, stats, gamma, beta);
           a1[j] += du;
           a2[j] = fmaf(du, xf - k.mean[j], a2[j]);
         }
@@ -615,7 +644,7 @@ __global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_bwd_kernel(const T
 #pragma unroll
   for (int j = 0; j < V; j++) {
     red[2 * j * RES_THREADS + tid] = a1[j];
-    red[(2 * j + 1) * RES_THREADS + tid] = a2[j] * rstd;
+    red[(2 * j + 1) * RES_THREADS + tid] = fmaf(-lo, a1[j], a2[j]) * rstd;
   }
   __syncthreads();
   // pixel rows: 16 lanes to a channel and sum
@@ -660,7 +689,7 @@ __global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_bwd_kernel(const T
   __syncthreads();
   if (!on) return;
   const float2 m = coef[cv * V / s.Cg];
-  const float q1 = rstd * m.x, q2 = rstd * rstd * m.y;
+  const float q2 = rstd * rstd * m.y, q1 = fmaf(-lo, q2, rstd * m.x);
 #pragma unroll
   for (int i = 0; i < NV; i++) {
     const int p = pr + i * s.PR;
@@ -669,7 +698,7 @@ __global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_bwd_kernel(const T
 #pragma unroll
       for (int j = 0; j < V; j++) {
         const float xf = to_f32(vx[i].t[j]);
-        const float du = du_of<ACT>(xf, to_f32(vd[i].t[j]), k.mean[j], k.a[j], k.beta[j], c + j, s.Cg, stats, gamma);
+        const float du = du_of<ACT>(xf, to_f32(vd[i].t[j]), k.mean[j], k.a[j], k.beta[j], c + j, s.Cg, stats, gamma, beta);
         o.t[j] = from_f32<T>(fmaf(du, k.a[j], -fmaf(xf - k.mean[j], q2, q1)));
       }
       *(typename Bits<T, V>::type*)(dx + base + (int64_t)p * s.C) = o.u;
@@ -841,7 +870,7 @@ void launch_fwd(const T* x, const Shape& s, int B, const float* gamma, const flo
   else if (V >= 4 && s.Cg % (V / 2) == 0) sum(std::integral_constant<int, (V >= 4 ? V / 2 : 1)>());
   else sum(std::integral_constant<int, 1>());
   const bool fold = (s.parts == 1 ? s.gps : 1) <= FOLD_GROUPS && s.chunks * s.parts <= FOLD_ROWS;
-  if (!fold) gn_stats_kernel<<<dim3(s.G, B), 64, 0, st>>>(sums, s.chunks * s.parts, s.G, (double)s.HW * s.Cg, eps, stats);
+  if (!fold) gn_stats_kernel<T><<<dim3(s.G, B), 64, 0, st>>>(x, s, sums, s.chunks * s.parts, s.G, (double)s.HW * s.Cg, eps, stats);
   with_act(act, [&](auto a) {
     constexpr int ACT = decltype(a)::value;
     if (fold) gn_apply_kernel<T, V, ACT, true><<<grid, GN_THREADS, 0, st>>>(x, s, sums, eps, stats, gamma, beta, y);
