@@ -312,7 +312,10 @@ __device__ __forceinline__ float du_of(float x, float dy, float mean, float a, f
 
 // rows[b][chunk][2][C] = (sum du, sum du xh) over the chunk's pixels.  Per channel, not per group, since dgamma and dbeta
 // need them so and the group's means follow from them.  16x32x512^2 bf16 with ReLU (537 MB) in 130 us, 4.1 TB/s (it starts on
-// the write-back of y's gradient).  Float32 within a thread (a few hundred terms), 64 bits from there on.
+// the write-back of y's gradient).  Float32 over the BWD_RUN pixels at most that a thread walks (plan cuts the chunks so: sums
+// of thousands of terms would be 10^-5 off) and pairwise over the workgroup's pixel rows, stored as float32; 64 bits over the
+// chunks and samples.
+constexpr int BWD_RUN = 64;
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(GN_THREADS) void gn_bwd_sums_kernel(const T* __restrict__ x, const T* __restrict__ dy, Shape s,
                                                                  const double2* __restrict__ stats_all,
@@ -595,7 +598,8 @@ __global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_kernel(const T* __
   }
 }
 
-// Backward of a resident slab: dx, and chan[b][2][C] for gn_bwd_finish_kernel.  16x512x32^2 bf16 with SiLU (50 MB) in 21 us.
+// Backward of a resident slab: dx, and chan[b][2][C] for gn_bwd_finish_kernel.  Its sums are float32 in short runs: at most 16
+// pixels in a thread, 32 and a tree of 16 lanes over the pixel rows, 32 and a tree of 64 over a group's channels.  16x512x32^2 bf16 with SiLU (50 MB) in 21 us.
 template <typename T, int V, int NV, int ACT>
 __global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_bwd_kernel(const T* __restrict__ x, const T* __restrict__ dy,
                                                                          Shape s, int B, const double2* __restrict__ stats_all,
@@ -709,6 +713,8 @@ __global__ __launch_bounds__(RES_THREADS, 2) void gn_resident_bwd_kernel(const T
 // ---------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------
+constexpr int64_t FWD_RUN = (int64_t)1 << 40;           // (its sums are 64-bit: no limit)
+
 // Slabs for vectors of V channels; false when they would not start on a vector.
 bool plan_slabs(Shape& s, int V) {
   if (s.C % V) return false;
@@ -740,8 +746,8 @@ bool plan_slabs(Shape& s, int V) {
 }
 
 // The widest vector that the channel count, the slabs and the tensors' addresses allow; chunks so that the launch
-// fills the chip eight times over but a thread still walks 4 pixels (one round of its loads).
-int plan(Shape& s, int B, int64_t HW, int C, int G, int esize, uintptr_t addr) {
+// fills the chip eight times over but a thread still walks 4 pixels (one round of its loads), and `run` at most.
+int plan(Shape& s, int B, int64_t HW, int C, int G, int esize, uintptr_t addr, int64_t run) {
   s.HW = HW;
   s.C = C;
   s.G = G;
@@ -753,6 +759,7 @@ int plan(Shape& s, int B, int64_t HW, int C, int G, int esize, uintptr_t addr) {
   int64_t want = (2048 + (int64_t)B * s.slabs - 1) / ((int64_t)B * s.slabs);
   if (want > most) want = most;
   if (want < 1) want = 1;
+  if (HW > want * s.PR * run) want = (HW + s.PR * run - 1) / (s.PR * run);
   s.ppc = (HW + want - 1) / want;
   s.chunks = (int)((HW + s.ppc - 1) / s.ppc);
   return V;
@@ -926,7 +933,7 @@ size_t fwd_bytes(int dtype, int B, int64_t HW, int C, int G) {
   size_t most = 0;
   for (uintptr_t addr = 2; addr <= 16; addr *= 2) {
     Shape s;
-    plan(s, B, HW, C, G, dtype == MIS_BF16 ? 2 : 4, addr);
+    plan(s, B, HW, C, G, dtype == MIS_BF16 ? 2 : 4, addr, FWD_RUN);
     const size_t n = (size_t)B * s.chunks * s.parts * s.G * sizeof(double2);
     if (n > most) most = n;
   }
@@ -937,7 +944,7 @@ size_t bwd_rows_bytes(int dtype, int B, int64_t HW, int C, int G) {
   size_t most = 0;
   for (uintptr_t addr = 2; addr <= 16; addr *= 2) {
     Shape s;
-    plan(s, B, HW, C, G, dtype == MIS_BF16 ? 2 : 4, addr);
+    plan(s, B, HW, C, G, dtype == MIS_BF16 ? 2 : 4, addr, BWD_RUN);
     const size_t n = (size_t)B * s.chunks * 2 * C * sizeof(float);
     if (n > most) most = n;
   }
@@ -966,7 +973,7 @@ int mis_group_norm_act_fwd(const void* x, int dtype, int B, int64_t HW, int C, i
   const uintptr_t addr = (uintptr_t)x | (uintptr_t)y | 16;
   int V;
   const int nv = plan_resident(s, V, B, HW, C, G, es, addr, RES_FWD);
-  if (!nv) V = plan(s, B, HW, C, G, es, addr);
+  if (!nv) V = plan(s, B, HW, C, G, es, addr, FWD_RUN);
   with_vector(dtype, V, [&](auto* t, auto v) {
     typedef std::remove_pointer_t<decltype(t)> T;
     if (nv)
@@ -999,7 +1006,7 @@ int mis_group_norm_act_bwd(const void* x, const void* dy, int dtype, int B, int6
   const uintptr_t addr = (uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx | 16;
   int V;
   const int nv = plan_resident(s, V, B, HW, C, G, es, addr, RES_BWD);
-  if (!nv) V = plan(s, B, HW, C, G, es, addr);
+  if (!nv) V = plan(s, B, HW, C, G, es, addr, BWD_RUN);
   BwdBuffers w;
   char* ws = (char*)workspace;
   w.rows = (float*)ws;

@@ -78,3 +78,20 @@ def test_spread_far_smaller_than_the_mean(shape, G, act):
     """Values over 64 steps of the float32 grid: a mean rounded to float32 is off by up to half a step, 1/37 of the spread, and
     E[x^2] - mean^2 in 64 bits by 1e-5 of itself."""
     _check(_far(shape, G, 0, shape[1]), G, act, 1e-14, 5)
+
+
+@pytest.mark.parametrize("C,H,W", [(129, 1500, 1400), (33, 3000, 2500), (8, 6000, 9000)])
+def test_bias_gradient_of_long_sums(C, H, W):
+    """Every pixel of a channel adds the same du, silu'(beta): dbias is the number of pixels times that.  At most 64 float32
+    additions in a row, 8 over the pixel rows of a workgroup, two roundings; one float32 sum of a thread's whole share (500 and
+    1000 terms of one size, whose roundings go one way) is 7e-6 off, 110 h32."""
+    from medical_image_segmentation_amd import functional as F_
+    b = torch.linspace(-1.0, 3.0, C, device=DEV, requires_grad=True)
+    grad = []
+    for h, w in ((1, 1), (H, W)):
+        x = torch.zeros(1, C, h, w, device=DEV, dtype=torch.bfloat16).contiguous(memory_format=torch.channels_last)
+        y = F_.group_norm_act(x, 1, None, b, activation="silu")
+        grad += torch.autograd.grad(y, [b], torch.ones_like(y))
+    one, many = grad[0].double(), grad[1].double()
+    err = ((many - H * W * one) / (H * W * one)).abs()
+    assert float(err.max()) <= 74 * H32, float(err.max())
