@@ -6,7 +6,10 @@
 // All products have one form, out[q][p] = sum over r of P(p, r) Q(q, r): the index p that is contiguous in the output
 // takes the matrix instruction's row operand, so that a lane's accumulators are consecutive elements of one output row.
 // Accumulation is float32; dz is rounded to the tensors' type once, as the operand of its two products (db is summed
-// from the unrounded values).
+// from the unrounded values).  In bf16 that is the price of the matrix instructions: they take no wider operand, and dz as a
+// sum of two bf16 would double both products and dz's bytes (16384x512 -> 2048, training, 225 us: by their times about 90 more).
+// dx and dW are then off from the exact ones by two roundings in place of one, 1.4 times as far in norm (0.0023 against 0.0017
+// for that product).
 #include "act.h"
 #include "common.h"
 #include "reduce.h"
@@ -210,10 +213,11 @@ template <int N> __device__ __forceinline__ void wait_and_meet() {
 #endif
 }
 
-// Measured, bf16: 8192x4096 -> 4096 with ReLU and residual 237 us, 1.16 PFLOP/s with the 256-edge: the matrix units are busy
-// 60 % of the time at 2.04 GHz and no LDS bank conflicts; power holds the clock there.  With sums of a few hundred the
-// epilogue's stores, which the workgroups of a round make at the same time, take as long as the products: 16384x512 -> 2048
-// with GELU 60 us (570 TFLOP/s), dz 77, dx 43 (800), dW 46 + 9 for the join.  float32: 4551x100 -> 252 in 12 us.
+// Measured, bf16: 8192x4096 -> 4096 with ReLU and residual 237 us, 1.16 PFLOP/s with the 256-edge: the matrix units are busy in
+// 54 % of the cycles, at 2.02 GHz; of the waves' cycles 33 % go to waits (the barrier of a stage and its loads), 47 % to waiting
+// for an issue slot, no LDS bank conflicts.  With sums of a few hundred the epilogue's stores, which the workgroups of a round
+// make at the same time, take as long as the products: 16384x512 -> 2048 with GELU 60 us (570 TFLOP/s), dz 77, dx 43 (800), dW
+// 46 + 9 for the join.  float32: 4551x100 -> 252 in 12 us.
 template <typename T, int TP, int TQ, int WP, int WQ, int STAGES, bool PTR, bool QTR, int MODE, bool WIDE>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void lin_tile_kernel(Operand<T> P, Operand<T> Q, int64_t R, Grid grid,
                                                                    Epilogue<T> e) {
@@ -406,8 +410,10 @@ __device__ __forceinline__ void any_stage(const Operand<T>& o, int row0, int64_t
   }
 }
 
-// Bound by its element loads: a stage of 128 bytes takes 2 to 6 us where the staged kernel takes 0.2 to 0.5; for products
-// too small to pay for padded copies (4x25 -> 678: 6 us).
+// Bound by its element loads: a stage of 128 bytes takes 2 to 6 us where the staged kernel takes 0.2 to 0.5.  For products
+// too small to pay for padded copies (4x25 -> 678: 6 us), and for rows that are whole 16-byte chunks long but start or step off
+// 16 bytes, which get no copy whatever their size: 8192x4096 -> 4096 bf16 from rows three elements off takes 5.9 ms, 0.25 from a
+// contiguous copy.
 template <typename T, int MODE>
 __global__ __launch_bounds__(256) void lin_any_kernel(Operand<T> P, Operand<T> Q, int64_t R, int64_t r_per_split, Epilogue<T> e) {
   __shared__ __attribute__((aligned(16))) T tp[ANY_T][ANY_PITCH], tq[ANY_T][ANY_PITCH];
@@ -558,7 +564,7 @@ __global__ __launch_bounds__(FEW ? 256 : 1024) void lin_join_kernel(const float*
 }
 
 // dst [rows][ld_dst] = src [rows][cols] with zeros behind each row, 16 bytes a thread: operands whose rows are not whole
-// 16-byte chunks are brought into that form once a call.
+// 16-byte chunks long are brought into that form once a call.
 template <typename T>
 __global__ __launch_bounds__(256) void lin_pad_kernel(const T* __restrict__ src, int64_t ld, int64_t rows, int cols, int ld_dst,
                                                       T* __restrict__ dst) {
@@ -647,6 +653,8 @@ struct Cut {
 // workgroup, at the time a load takes; for a split sum the second launch, and the parts written and read.  The constants
 // are fitted to 160 products of 1 to 10^6 rows and 24 to 4096 columns, forward and the three backward ones, bf16 and
 // float32, each measured in all cuts: the choice is 2 % slower than the best cut on average, 29 % at worst (14 us for 11).
+// It ranks cuts; as a time it is short where the epilogue is dear, for which it has no term (16384x512 -> 2048: 31 us, measured 45
+// bare and 60 with GELU; 4551x104 -> 252 float32: 3.6 and 11.7).
 // ANY64's are from nine odd products (a stage of 2.2 to 6.4 us alone and 2 to 3.5 shared, in either type): 1000 x 2001 -> 1001
 // in bf16 takes 132 us there and 27 as padded copies, 25 x 1087 -> 15 in float32 75 and 15; 4 x 25 -> 678 stays at 6.
 Cut pick_cut(int esize, bool staged, int64_t p, int64_t q, int64_t r) {
@@ -774,7 +782,7 @@ const T* pad(const T* src, int64_t rows, int64_t cols, int64_t ld, T* dst, hipSt
   return dst;
 }
 
-// The buffers of a call, in the order the code below uses them.  Rows that are not whole 16-byte chunks get a padded copy
+// The buffers of a call, in the order the code below uses them.  Rows that are not whole 16-byte chunks long get a padded copy
 // where that pays; sizes are for the case that it does.
 template <typename T> struct Buffers {
   T *x, *w, *z;
