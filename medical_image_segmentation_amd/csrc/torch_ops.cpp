@@ -235,22 +235,23 @@ class Layouts {
   std::vector<One> kept_;
 };
 
-// Whether the values of an optimizer's `state` are still these dicts, in this order, and hold these tensors (as many to a dict
-// as there are keys; None: no such entry): a user may clear the state, or put other dicts or tensors in its place.
-bool state_holds(const pybind11::dict& state, const pybind11::list& dicts, const pybind11::tuple& keys,
-                 const pybind11::list& tensors) {
-  const Py_ssize_t n = PyList_GET_SIZE(dicts.ptr()), k = PyTuple_GET_SIZE(keys.ptr());
-  if (PyDict_Size(state.ptr()) != n || PyList_GET_SIZE(tensors.ptr()) != n * k) return false;
-  PyObject *key, *value;
-  Py_ssize_t at = 0;
+// Whether the values of an optimizer's `state` are still these dicts, in this order, and hold these entries one dict after the
+// other (None: any): a user may clear the state, or put other dicts or tensors in its place.  Dicts keep their order, so
+// nothing is looked up by its key.
+bool state_holds(const pybind11::dict& state, const pybind11::list& dicts, const pybind11::list& entries) {
+  const Py_ssize_t n = PyList_GET_SIZE(dicts.ptr()), m = PyList_GET_SIZE(entries.ptr());
+  if (PyDict_Size(state.ptr()) != n) return false;
+  PyObject *key, *value, *entry;
+  Py_ssize_t at = 0, e = 0;
   for (Py_ssize_t i = 0; PyDict_Next(state.ptr(), &at, &key, &value); i++) {
     if (value != PyList_GET_ITEM(dicts.ptr(), i) || !PyDict_Check(value)) return false;
-    for (Py_ssize_t j = 0; j < k; j++) {
-      PyObject* held = PyDict_GetItem(value, PyTuple_GET_ITEM(keys.ptr(), j));
-      if ((held ? held : Py_None) != PyList_GET_ITEM(tensors.ptr(), i * k + j)) return false;
+    for (Py_ssize_t in = 0; PyDict_Next(value, &in, &key, &entry); e++) {
+      if (e >= m) return false;
+      PyObject* held = PyList_GET_ITEM(entries.ptr(), e);
+      if (held != Py_None && held != entry) return false;
     }
   }
-  return true;
+  return e == m;
 }
 
 // The pointers [parameter, gradient, parameter, ...] of parameters whose gradients lie in the same memory order, type and

@@ -466,10 +466,10 @@ class _Plan8:
     def keep(self, state):
         """Takes note of the state that the buffers serve: `holds` says whether it is still that one."""
         self.states = list(state.values())
-        self.held = [s.get(k) for s in self.states for k in AdamW8._STATE]
+        self.held = [v if k in AdamW8._STATE else None for s in self.states for k, v in s.items()]
 
     def holds(self, state):
-        return F_._native().state_holds(state, self.states, AdamW8._STATE, self.held)
+        return F_._native().state_holds(state, self.states, self.held)
 
     def table(self, groups, state, params):
         """The launch tables for `params`, the parameters that have a gradient now."""
