@@ -92,8 +92,8 @@ template <typename T> __device__ __forceinline__ double first_of(const T* __rest
 // sums[b][chunk*parts + part][g] = (sum d, sum d*d) over the chunk's pixels and the slab's channels of g.
 // U: channels of a vector that are sure to share a group (a power of two that divides V and the group), so a thread holds
 // V/U pairs of sums and not V: few enough registers for eight waves to a SIMD, which the stream of loads needs.
-// Bound by HBM: 16x32x512^2 bf16 (268 MB) in 72 us behind a kernel whose output is still being written back, 3.7 TB/s; its
-// loop alone reads 7 TB/s.
+// Bound by HBM: 16x32x512^2 bf16 (268 MB) in 74 us (72 without K) behind a kernel whose output is still being written back, 3.6
+// TB/s; its loop alone reads 7 TB/s.
 template <typename T, int V, int U>
 __global__ __launch_bounds__(GN_THREADS) void gn_sums_kernel(const T* __restrict__ x, Shape s, double2* __restrict__ sums) {
   constexpr int N = V / U;
@@ -311,7 +311,7 @@ __device__ __forceinline__ float du_of(float x, float dy, float mean, float a, f
 }
 
 // rows[b][chunk][2][C] = (sum du, sum du xh) over the chunk's pixels.  Per channel, not per group, since dgamma and dbeta
-// need them so and the group's means follow from them.  16x32x512^2 bf16 with ReLU (537 MB) in 130 us, 4.1 TB/s (it starts on
+// need them so and the group's means follow from them.  16x32x512^2 bf16 with ReLU (537 MB) in 131 us, 4.1 TB/s (it starts on
 // the write-back of y's gradient).  Float32 over the BWD_RUN pixels at most that a thread walks (plan cuts the chunks so: sums
 // of thousands of terms would be 10^-5 off) and pairwise over the workgroup's pixel rows, stored as float32; 64 bits over the
 // chunks and samples.

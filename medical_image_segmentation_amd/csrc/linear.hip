@@ -216,8 +216,8 @@ template <int N> __device__ __forceinline__ void wait_and_meet() {
 // Measured, bf16: 8192x4096 -> 4096 with ReLU and residual 237 us, 1.16 PFLOP/s with the 256-edge: the matrix units are busy in
 // 54 % of the cycles, at 2.02 GHz; of the waves' cycles 33 % go to waits (the barrier of a stage and its loads), 47 % to waiting
 // for an issue slot, no LDS bank conflicts.  With sums of a few hundred the epilogue's stores, which the workgroups of a round
-// make at the same time, take as long as the products: 16384x512 -> 2048 with GELU 60 us (570 TFLOP/s), dz 77, dx 43 (800), dW
-// 46 + 9 for the join.  float32: 4551x100 -> 252 in 12 us.
+// make at the same time, take as long as the products: 16384x512 -> 2048 with GELU 62 us (550 TFLOP/s), dz 79, dx 42 (810),
+// dW 46 + 9 for the join.  float32: 4551x100 -> 252 in 12 us.
 template <typename T, int TP, int TQ, int WP, int WQ, int STAGES, bool PTR, bool QTR, int MODE, bool WIDE>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void lin_tile_kernel(Operand<T> P, Operand<T> Q, int64_t R, Grid grid,
                                                                    Epilogue<T> e) {
@@ -654,7 +654,7 @@ struct Cut {
 // are fitted to 160 products of 1 to 10^6 rows and 24 to 4096 columns, forward and the three backward ones, bf16 and
 // float32, each measured in all cuts: the choice is 2 % slower than the best cut on average, 29 % at worst (14 us for 11).
 // It ranks cuts; as a time it is short where the epilogue is dear, for which it has no term (16384x512 -> 2048: 31 us, measured 45
-// bare and 60 with GELU; 4551x104 -> 252 float32: 3.6 and 11.7).
+// bare and 62 with GELU; 4551x104 -> 252 float32: 3.6 and 11.7).
 // ANY64's are from nine odd products (a stage of 2.2 to 6.4 us alone and 2 to 3.5 shared, in either type): 1000 x 2001 -> 1001
 // in bf16 takes 132 us there and 27 as padded copies, 25 x 1087 -> 15 in float32 75 and 15; 4 x 25 -> 678 stays at 6.
 Cut pick_cut(int esize, bool staged, int64_t p, int64_t q, int64_t r) {
