@@ -598,6 +598,7 @@ class _CapturedStep8:
         self.plan = optimizer._flat()
         self.table = _Table8(self.plan, optimizer.param_groups, optimizer.state, self.params)
         self.addresses = [p.data_ptr() for p in self.table.order]
+        self.options = self._options()
         dev, n, r = self.plan.device, len(self.table.order), max(len(self.table.runs), 1)
         self.rows_host = torch.empty((n, 5), dtype=torch.int64).pin_memory()
         self.descs = torch.empty((n, 5), dtype=torch.int64, device=dev)
@@ -608,7 +609,14 @@ class _CapturedStep8:
         self.dyn = torch.zeros((r, self.WIDTH), dtype=torch.uint8, device=dev)
         self.norm = None
 
+    def _options(self):
+        """What a launch holds fast (learning rate and weight decay come from the device buffer)."""
+        return [(tuple(g["betas"]), g["eps"], g["seed"]) for g, _, _ in self.table.runs]
+
     def prepare(self):
+        if self._options() != self.options:
+            raise RuntimeError("betas, eps or seed changed after the capture (a scheduler that cycles momentum does that): capture "
+                               "the step again")
         if self.optimizer._plan is not self.plan or not self.plan.holds(self.optimizer.state):
             raise RuntimeError("the optimizer's state was replaced after the capture: capture the step again")
         if not self.plan.matches(self.plan.params) or [p.data_ptr() for p in self.table.order] != self.addresses:

@@ -186,3 +186,18 @@ def test_a_checkpoint_of_a_channels_last_model():
     with pytest.raises(RuntimeError, match="parameter 0 is now"):
         oc.load_state_dict(saved)
     assert not oc.state
+
+
+@pytest.mark.parametrize("change", [dict(betas=(0.8, 0.99)), dict(eps=1e-6), dict(seed=5)])
+def test_a_captured_step_refuses_options_that_its_launches_hold_fast(change):
+    """lr and weight_decay are read before every replay; the others are arguments of the captured launches."""
+    m, opt, step, x = _captured()
+    group = opt.param_groups[0]
+    kept, taken = {k: group[k] for k in change}, opt.state[m.narrow.weight]["step"]
+    group.update(change)
+    with pytest.raises(RuntimeError, match="changed after the capture"):
+        step(x, x)
+    assert opt.state[m.narrow.weight]["step"] == taken
+    group.update(kept, lr=1e-4, weight_decay=0.0)
+    step(x, x)
+    assert opt.state[m.narrow.weight]["step"] == taken + 1
