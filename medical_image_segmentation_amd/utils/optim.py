@@ -262,16 +262,19 @@ def _dense(t):
 
 def _layout(p):
     """(shape, dimensions by falling stride): which element lies at which place of a dense tensor's memory."""
-    dims = [d for d in range(p.dim()) if p.shape[d] != 1] if p.numel() else []
-    return tuple(p.shape), tuple(sorted(dims, key=lambda d: -p.stride(d)))
+    shape = tuple(p.shape)
+    dims = [d for d, n in enumerate(shape) if n != 1] if 0 not in shape else []
+    if len(dims) > 1 and not p.is_contiguous():
+        dims.sort(key=lambda d: -p.stride(d))
+    return shape, tuple(dims)
 
 
 def _check_layout(i, p, s):
     """The codes of state `s` follow the memory of the tensor they were made for: they mean nothing in another order.  Without a
     record of it they are taken for row-major."""
-    shape, order = _layout(p)
-    made = s.get("layout", (shape, sorted(order)))
-    if (tuple(made[0]), tuple(made[1])) != (shape, order):
+    shape, order = now = _layout(p)
+    made = s.get("layout") or (shape, sorted(order))
+    if made != now and (tuple(made[0]), tuple(made[1])) != now:
         raise RuntimeError(f"AdamW8: parameter {i} is now {shape} with strides {p.stride()}, its moments were made for shape "
                            f"{tuple(made[0])} with the dimensions {tuple(made[1])} by falling stride: convert the model back, or "
                            "delete the parameter's state to begin again")
@@ -351,21 +354,23 @@ class AdamW8(torch.optim.Optimizer):
         params = self._params()
         for i, p in zip(names, params):
             if i in states:
-                self.state[p].update({k: states[i][k].reshape(-1) for k in self._STATE}, step=int(states[i]["step"]),
-                                     layout=_layout(p))
+                self.state[p].update({k: states[i][k] for k in self._STATE}, step=int(states[i]["step"]))
         self._plan = None
         if all(p.is_cuda for p in params) and len({p.device for p in params}) == 1:
-            self._flat()
+            self._flat(params, checked=True)
         else:                                      # nothing of the given tensors is kept
             for s in self.state.values():
-                s.update({k: s[k].clone() for k in self._STATE if k in s})
+                s.update({k: s[k].reshape(-1).clone() for k in self._STATE if k in s})
+            for p in params:
+                if p in self.state:
+                    self.state[p]["layout"] = _layout(p)
 
     def _params(self):
         return [p for g in self.param_groups for p in g["params"]]
 
-    def _flat(self, params=None):
+    def _flat(self, params=None, checked=False):
         """The flat moment buffers, laid out over all parameters (`params`, where the caller has their list); state[p] holds
-        views of them."""
+        views of them.  checked: what the state holds has been looked at."""
         params = params or self._params()
         plan = self._plan
         if plan is not None and plan.matches(params) and plan.holds(self.state):
@@ -374,7 +379,7 @@ class AdamW8(torch.optim.Optimizer):
         if len(devs) != 1 or next(iter(devs)).type != "cuda":
             raise RuntimeError(f"AdamW8 needs all parameters on one GPU, got {sorted(map(str, devs))}")
         for i, p in enumerate(params):
-            if self.state.get(p):
+            if not checked and self.state.get(p):
                 _check_layout(i, p, self.state[p])
                 _check_codes(i, p.numel(), self.state[p])
         plan = self._plan = _Plan8(params, next(iter(devs)))
@@ -387,7 +392,7 @@ class AdamW8(torch.optim.Optimizer):
                 if k in s:                        # (codes behind the last element stay zero)
                     n = p.numel() if v is views[0] or v is views[2] else v[i].numel()
                     to.append(v[i][:n])
-                    given.append(s[k].reshape(-1)[:n])
+                    given.append((s[k] if s[k].dim() == 1 else s[k].reshape(-1))[:n])
                 s[k] = v[i]
             s["step"] = int(s.get("step", 0))
             s["layout"] = _layout(p)
