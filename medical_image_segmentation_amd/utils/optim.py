@@ -343,8 +343,8 @@ class AdamW8(torch.optim.Optimizer):
         for i, p in zip(names, self._params()):        # (before anything is replaced; torch checks the groups' lengths)
             s = state_dict["state"].get(i)
             if s is not None:
-                if not _check_codes(i, p.numel(), s):
-                    raise ValueError(f"not an AdamW8 state: parameter {i} has no {self._STATE[0]}")
+                if not _check_codes(i, p.numel(), s) or "step" not in s:
+                    raise ValueError(f"not an AdamW8 state: parameter {i} has no {'step' if 'exp_avg' in s else 'exp_avg'}")
                 _check_layout(i, p, s)
         # (the codes go past torch's loading, which would take them through the parameters' floating-point type)
         states = state_dict["state"]
@@ -382,7 +382,7 @@ class AdamW8(torch.optim.Optimizer):
             if not checked and self.state.get(p):
                 _check_layout(i, p, self.state[p])
                 _check_codes(i, p.numel(), self.state[p])
-        plan = self._plan = _Plan8(params, next(iter(devs)))
+        plan = _Plan8(params, next(iter(devs)))
         views = [buf.split([(b1 - b0) * w for b0, b1 in plan.spans] + [buf.numel() - plan.blocks * w])
                  for buf, w in zip(plan.buffers, (BLOCK8, 1, BLOCK8, 1))]
         to, given = [], []
@@ -393,12 +393,13 @@ class AdamW8(torch.optim.Optimizer):
                     n = p.numel() if v is views[0] or v is views[2] else v[i].numel()
                     to.append(v[i][:n])
                     given.append((s[k] if s[k].dim() == 1 else s[k].reshape(-1))[:n])
-                s[k] = v[i]
-            s["step"] = int(s.get("step", 0))
-            s["layout"] = _layout(p)
         if to:
             torch._foreach_copy_(to, given)
+        for i, p in enumerate(params):             # (nothing of the old state is replaced before all of it is copied)
+            s = self.state[p]
+            s.update({k: v[i] for k, v in zip(self._STATE, views)}, step=int(s.get("step", 0)), layout=_layout(p))
         plan.keep(self.state)
+        self._plan = plan
         return plan
 
     def moments(self, p=None):

@@ -201,3 +201,21 @@ def test_a_captured_step_refuses_options_that_its_launches_hold_fast(change):
     group.update(kept, lr=1e-4, weight_decay=0.0)
     step(x, x)
     assert opt.state[m.narrow.weight]["step"] == taken + 1
+
+
+def test_a_state_that_cannot_be_copied_is_left_as_it_was(monkeypatch):
+    """Laying the buffers out again goes through a copy of the old ones; where it fails, the old state is still there."""
+    from medical_image_segmentation_amd.utils.optim import AdamW8
+    p, q = _params([300], torch.float32, 51)[0], _params([40], torch.float32, 52)[0]
+    opt = AdamW8([p], **HP)
+    _grads([p], 1)
+    opt.step()
+    before = [t.clone() for t in opt.moments(p)]
+    opt.add_param_group(dict(params=[q]))
+    with monkeypatch.context() as m:
+        def fails(*args):
+            raise RuntimeError("no memory")
+        m.setattr(torch, "_foreach_copy_", fails)
+        with pytest.raises(RuntimeError, match="no memory"):
+            opt.step()
+    assert opt.state[p]["step"] == 1 and all(torch.equal(a, b) for a, b in zip(before, opt.moments(p)))
